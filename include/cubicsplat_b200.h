@@ -378,6 +378,84 @@ CS_API int cs_adam_step(float *params, float *grads, float *exp_avg, float *exp_
                  float eps, int32_t *step, void *workspace, int32_t clear_grads, void *stream);
 
 /* --------------------------------------------------------------------------
+ * AdamW over many tensors at once
+ *
+ * Host arrays of tensors in, as few launches as the kernels' parameter tables
+ * allow out (several hundred tensors a launch).  The arrays are read before
+ * the call returns; nothing is kept.  A tensor is its elements in storage
+ * order: parameter, gradient and moments have one layout.  No written buffer
+ * may overlap another buffer of the call.
+ * ------------------------------------------------------------------------ */
+
+#define CS_F32 0
+#define CS_BF16 1
+#define CS_F16 2
+
+#define CS_ADAMW_MAX_GROUPS 16
+#define CS_ADAMW8_BLOCK 256 /* elements that share a scale byte */
+
+typedef struct cs_adamw_tensor {
+  void *param;                /* dtype */
+  const void *grad;           /* dtype */
+  void *exp_avg;              /* float, or uint8_t codes (cs_adamw8_*) */
+  void *exp_avg_sq;           /* float, or uint8_t codes (cs_adamw8_*) */
+  uint8_t *exp_avg_scales;    /* cs_adamw8_*: one byte per started block of 256 elements */
+  uint8_t *exp_avg_sq_scales; /* likewise */
+  int64_t numel;
+  int32_t dtype; /* CS_F32, CS_BF16 or CS_F16, of param and grad */
+  int32_t group; /* index into the call's groups */
+} cs_adamw_tensor;
+
+typedef struct cs_adamw_group {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;           /* this step's number, from 1 (read where coef is NULL) */
+  const float *lr_device; /* device scalar that replaces lr, or NULL */
+} cs_adamw_group;
+
+/* One AdamW step: g' = *grad_scale * g (grad_scale a device scalar, NULL for 1),
+ * m = b1 m + (1-b1) g', v = b2 v + (1-b2) g'^2,
+ * p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps).
+ * coef NULL: t is each group's step; else the device array that
+ * cs_adamw_advance wrote for these groups. */
+CS_API int cs_adamw_step(const cs_adamw_tensor *tensors, int32_t count,
+                  const cs_adamw_group *groups, int32_t num_groups, const float *coef,
+                  const float *grad_scale, void *stream);
+
+/* The same step with moments of one byte an element and one scale byte E for
+ * each block of 256: m is a sign, 4 exponent and 3 fraction bits, v 5 exponent
+ * and 3 fraction bits, both with gradual underflow, in units of 2^(E-127);
+ * E = 255 marks a block that is not finite.  Zeroed bytes stand for zero.  The
+ * bytes are rounded stochastically from a hash of (seed, t, place of the tensor
+ * in the array, element), so a call is reproducible. */
+CS_API int cs_adamw8_step(const cs_adamw_tensor *tensors, int32_t count,
+                   const cs_adamw_group *groups, int32_t num_groups, const float *coef,
+                   uint32_t seed, const float *grad_scale, void *stream);
+
+/* Values of 8-bit moments: param and grad point to the float outputs for m and
+ * v (both written), dtype is CS_F32, group 0. */
+CS_API int cs_adamw8_moments(const cs_adamw_tensor *tensors, int32_t count, void *stream);
+
+/* Advances each group's device step counter by one and writes coef (4 floats a
+ * group) for the step that follows, so that a captured step counts on replay. */
+CS_API int cs_adamw_advance(int64_t *const *steps, const cs_adamw_group *groups,
+                     int32_t num_groups, uint32_t seed, float *coef, void *stream);
+
+typedef struct cs_grad_tensor {
+  const void *data;
+  int64_t numel;
+  int32_t dtype;
+  int32_t reserved;
+} cs_grad_tensor;
+
+/* norm = sqrt of the sum of squares over all tensors, accumulated in double;
+ * scale (may be NULL) = min(1, max_norm / (norm + eps)), or 1 for max_norm <= 0.
+ * Workspace: cs_grad_norm_workspace_size(count) bytes, 8-byte aligned, in any
+ * state, not shared with a call that may run at the same time. */
+CS_API size_t cs_grad_norm_workspace_size(int32_t count);
+CS_API int cs_grad_norm(const cs_grad_tensor *tensors, int32_t count, double max_norm, double eps,
+                 float *norm, float *scale, void *workspace, void *stream);
+
+/* --------------------------------------------------------------------------
  * Closed control polygon -> ring of piecewise-Hermite cubics
  * ------------------------------------------------------------------------ */
 

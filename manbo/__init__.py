@@ -4,7 +4,8 @@ Same module paths and names as the reference's ``manbo`` (manbo/__init__.py:1-29
 for the render/optimise hot path: the cubic fill and stroke renderers, their
 per-stage operators, the ring-segment conversion, the MSE / PSNR / SSIM
 metrics, the Adan optimiser that train.py uses by default, the regularisation
-loss and the connected-component labelling.  The Gaussian renderer, outside
+loss and the connected-component labelling; and, beside the reference's names,
+an AdamW optimiser that moves all parameters in one launch.  The Gaussian renderer, outside
 that path, keeps its names so that imports succeed, and raises
 NotImplementedError when called.
 """
@@ -33,7 +34,7 @@ if not _importable("visual_debug"):
 
 from . import ops
 from .metric import mse_loss_tilelang, psnr, ssim
-from .optim import Adan
+from .optim import AdamW, Adan
 from .regularization import regularization_loss_tilelang
 from .tilelang_renderer import GsRenderFunction, GsRenderModule, gs_render, set_gs_profile_ctx_factory
 
@@ -44,6 +45,7 @@ __all__ = [
     "psnr",
     "ssim",
     "Adan",
+    "AdamW",
     "GsRenderFunction",
     "GsRenderModule",
     "set_gs_profile_ctx_factory",

@@ -3,12 +3,22 @@
 Hot-path operators (cubic fill / stroke renderer stages, tile bins, ring
 segments, metric kernels) run on the B200 sm_100a kernels, and so do the Adan
 step (train.py's default optimiser) and the 4-connected component labelling.
+The AdamW operators over many tensors (``adamw_step``, ``adamw8_step``,
+``grad_norm``) have no counterpart in the reference.
 The Gaussian renderer's operators are outside the B200 hot path, and the
 reference's per-term regularisation kernels have no counterpart (one launch
 computes every term of ``manbo.regularization_loss_tilelang``): their names
 exist so imports succeed, and calling them raises NotImplementedError.
 """
 from .._unavailable import unavailable
+from .adamw import (
+    ADAMW8_BLOCK,
+    adamw8_moments,
+    adamw8_state,
+    adamw8_step,
+    adamw_step,
+    grad_norm,
+)
 from .connected_components import (
     connected_components_labels_4_tilelang,
     connected_components_with_stats_4_tilelang,
@@ -95,6 +105,12 @@ __all__ = [
     "ssim_map_kernel",
     "reduce_sum_1d_tilelang",
     "adan_step_from_grad_tilelang",
+    "ADAMW8_BLOCK",
+    "adamw8_moments",
+    "adamw8_state",
+    "adamw8_step",
+    "adamw_step",
+    "grad_norm",
     "connected_components_labels_4_tilelang",
     "connected_components_with_stats_4_tilelang",
     "select_largest_component_center",

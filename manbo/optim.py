@@ -1,18 +1,27 @@
-"""Adan optimiser on the B200 step kernel (mirrors manbo/optim.py:10-190).
+"""Optimisers on the B200 step kernels: Adan (mirrors manbo/optim.py:10-190)
+and AdamW over all parameters at once.
 
-Same constructor, validation, state (``exp_avg``, ``exp_avg_sq``,
+``Adan`` has the same constructor, validation, state (``exp_avg``, ``exp_avg_sq``,
 ``exp_avg_diff``, ``neg_pre_grad`` per parameter), ``restart_opt`` and global
 gradient-norm clipping as the reference; every parameter's update is one
 ``cs_adan_step`` launch.  Like the reference, clipping (max_grad_norm > 0)
 reads the norm on the host, once per step.
+
+``AdamW`` (no counterpart in the reference) moves every parameter in one launch,
+with its moments in 32 bits or in 8 (manbo/ops/adamw.py), clips by the global
+gradient norm without reading it back, and can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import itertools
 import math
 
 import torch
 from torch.optim.optimizer import Optimizer
 
+from repo_b200 import _ext
+
+from .ops.adamw import adamw8_moments, adamw8_state, grad_norm
 from .ops.optim import adan_step_from_grad_kernel
 
 DEFAULT_TILELANG_THREADS = 256
@@ -118,4 +127,193 @@ class Adan(Optimizer):
         return loss
 
 
-__all__ = ["Adan"]
+_ADAMW_MAX_GROUPS = 16  # hyper-parameter groups of one launch
+
+
+class AdamW(Optimizer):
+    """Adam with decoupled weight decay, every parameter of a device in one launch.
+
+    ``state_bits`` 32 keeps ``exp_avg`` and ``exp_avg_sq`` as float32 in the
+    parameter's layout, 8 as one byte an element with a scale byte for each 256
+    elements (see ``manbo.ops.adamw8_step``; ``seed`` feeds its rounding).
+    ``max_grad_norm`` > 0 clips by the global norm of all gradients, which stays
+    on the device (``grad_norm`` holds the last one).  Parameters are float32,
+    bfloat16 or float16, non-overlapping and dense.
+
+    Steps are counted per parameter, from the first step at which it has a
+    gradient.  With ``capturable`` the count lives on the device, one counter for
+    the parameters of a group that get their first gradient in the same step, so
+    that a captured step counts on every replay; a group's ``lr`` may then be a
+    float32 device scalar that a schedule writes to.  Take one step before the
+    capture, so that the state exists.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, max_grad_norm: float = 0.0, state_bits: int = 32,
+                 capturable: bool = False, seed: int = 0):
+        if not 0.0 <= max_grad_norm:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        if isinstance(lr, torch.Tensor):
+            if not capturable:
+                raise ValueError("lr as a tensor needs capturable=True")
+        elif not 0.0 <= lr:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= eps:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        for i in range(2):
+            if not 0.0 <= betas[i] < 1.0:
+                raise ValueError(f"Invalid beta parameter at index {i}: {betas[i]}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      max_grad_norm=max_grad_norm, state_bits=state_bits,
+                                      capturable=capturable, seed=seed))
+        self.grad_norm = None
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("grad_norm", None)
+        for group in self.param_groups:
+            for key, value in self.defaults.items():
+                group.setdefault(key, value)
+
+    def _new_state(self, p, group, counters, capturing):
+        if capturing:
+            raise RuntimeError("AdamW: take one step before capturing, so that the state exists")
+        st = {}
+        if group["state_bits"] == 8:
+            (st["exp_avg"], st["exp_avg_scales"], st["exp_avg_sq"],
+             st["exp_avg_sq_scales"]) = adamw8_state(p)
+        else:
+            for k in ("exp_avg", "exp_avg_sq"):
+                st[k] = torch.zeros_like(p, dtype=torch.float32,
+                                         memory_format=torch.preserve_format)
+        if group["capturable"]:
+            if p.device not in counters:
+                counters[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+            st["step"] = counters[p.device]
+        else:
+            st["step"] = 0
+        return st
+
+    def _plan(self):
+        """{(device, state_bits): [(group, step, parameters)]} of this step, the
+        parameters of an entry at the same step."""
+        plan = {}
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        for group in self.param_groups:
+            cohorts, counters = {}, {}
+            if capturing and not group["capturable"]:
+                raise RuntimeError("AdamW: a captured step needs capturable=True")
+            eight = group["state_bits"] == 8
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if not p.is_cuda:
+                    raise ValueError("AdamW parameters must be CUDA tensors")
+                st = self.state[p]
+                if not st:
+                    st.update(self._new_state(p, group, counters, capturing))
+                if ("exp_avg_scales" in st) != eight:
+                    raise ValueError(f"AdamW state is not of state_bits={group['state_bits']}")
+                step = st["step"]
+                if isinstance(step, torch.Tensor) != bool(group["capturable"]):
+                    raise ValueError("AdamW state was made with another value of capturable")
+                key = (p.device, id(step) if group["capturable"] else step)
+                if key not in cohorts:
+                    cohorts[key] = (group, step, [])
+                    plan.setdefault((p.device, group["state_bits"]), []).append(cohorts[key])
+                cohorts[key][2].append(p)
+        return plan
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        plan = self._plan()
+        if not plan:
+            return loss
+        scale = None
+        if self.defaults["max_grad_norm"] > 0:
+            grads = [p.grad for parts in plan.values() for _, _, ps in parts for p in ps]
+            if len({g.device for g in grads}) > 1:
+                raise ValueError("max_grad_norm needs every parameter on one device")
+            self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
+        ext = _ext.load()
+        for (_, bits), parts in plan.items():
+            for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
+                some = parts[at:at + _ADAMW_MAX_GROUPS]
+                groups = [(len(ps), g["lr"], g["betas"][0], g["betas"][1], g["eps"],
+                           g["weight_decay"], step if g["capturable"] else step + 1)
+                          for g, step, ps in some]
+                params = [p for _, _, ps in some for p in ps]
+                grads = [p.grad for p in params]
+                states = [self.state[p] for p in params]
+                if bits == 8:
+                    ext.adamw8_step(params, grads, [s["exp_avg"] for s in states],
+                                    [s["exp_avg_scales"] for s in states],
+                                    [s["exp_avg_sq"] for s in states],
+                                    [s["exp_avg_sq_scales"] for s in states], groups,
+                                    some[0][0]["seed"] & 0xFFFFFFFF, scale)
+                else:
+                    ext.adamw_step(params, grads, [s["exp_avg"] for s in states],
+                                   [s["exp_avg_sq"] for s in states], groups, scale)
+                for s in states:
+                    if not isinstance(s["step"], torch.Tensor):
+                        s["step"] += 1
+        return loss
+
+    @torch.no_grad()
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of a parameter as new float32 tensors."""
+        st = self.state[p]
+        if "exp_avg_scales" not in st:
+            return st["exp_avg"].clone(), st["exp_avg_sq"].clone()
+        m, v = adamw8_moments([st["exp_avg"]], [st["exp_avg_scales"]], [st["exp_avg_sq"]],
+                              [st["exp_avg_sq_scales"]])
+        return m[0], v[0]
+
+    @torch.no_grad()
+    def restart_opt(self):
+        """Forget every moment and step count."""
+        self.state.clear()
+
+    def load_state_dict(self, state_dict):
+        """As the base class, except that moments keep their own types (the base
+        class casts them to the parameter's) and are copies of the given ones."""
+        super().load_state_dict({**state_dict, "state": {}})
+        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        own = [(p, g) for g in self.param_groups for p in g["params"]]
+        counters = {}
+        for i, (p, group) in zip(ids, own):
+            if i not in state_dict["state"]:
+                continue
+            st = {}
+            codes = state_dict["state"][i].get("exp_avg")
+            if codes is not None and codes.dtype == torch.uint8 and codes.stride() != p.stride():
+                raise ValueError("8-bit moments need the strides of the parameter they were "
+                                 "saved with (their blocks follow its storage)")
+            for k, x in state_dict["state"][i].items():
+                if k == "step":
+                    if not group["capturable"]:
+                        st[k] = int(x)
+                    else:  # parameters that shared a counter share the new one
+                        key = (id(group), id(x) if isinstance(x, torch.Tensor) else x, p.device)
+                        if key not in counters:
+                            counters[key] = torch.tensor(int(x), dtype=torch.int64,
+                                                         device=p.device)
+                        st[k] = counters[key]
+                elif isinstance(x, torch.Tensor):
+                    y = torch.empty_like(p, dtype=x.dtype) if x.shape == p.shape \
+                        else torch.empty_like(x, device=p.device)
+                    st[k] = y.copy_(x)
+                else:
+                    st[k] = x
+            self.state[p] = st
+
+
+__all__ = ["Adan", "AdamW"]

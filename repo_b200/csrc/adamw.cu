@@ -1,0 +1,823 @@
+// AdamW over many tensors at once (sm_100a): the global gradient norm with its
+// clip factor, the step with 32-bit moments, the step with 8-bit moments, and
+// the values of 8-bit moments.
+//
+// Every entry takes a host array of tensors.  Pointers, sizes, types and the
+// groups' hyper-parameters travel in the kernel's parameters (up to 32 KB), so
+// a call uploads nothing, keeps nothing, and can be captured in a CUDA graph;
+// one launch covers all tensors of a call up to the table's capacity.  A CTA
+// finds the tensor of its chunk by a binary search over the chunk prefix.
+//
+// All of it is bound by HBM: the step moves 28 B an element (float32) or 22 B
+// (16-bit parameters), with 8-bit moments 16 B or 10 B.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "cs_common.cuh"
+
+namespace cs {
+
+constexpr int kChunkThreads = 256;
+constexpr int kPerThread = 8;
+constexpr int kBlock8 = CS_ADAMW8_BLOCK;                  // elements of a scale block: one warp's
+constexpr int kChunk = kChunkThreads * kPerThread;        // elements of a CTA's chunk
+static_assert(kBlock8 == 32 * kPerThread, "a warp holds one scale block");
+constexpr int64_t kMaxNumel = int64_t(1) << 40;
+constexpr int kMaxTensors = 1 << 22;                      // places that fit an entry's word
+
+// ---------------------------------------------------------------------------
+// Tables in kernel parameters
+
+struct AdamGroup {
+  float b1, omb1, b2, omb2, eps, lr, wd, ibc1, rbc2;  // ibc1 = 1/(1-b1^t), rbc2 = 1/sqrt(1-b2^t)
+  uint32_t key;                                       // of the stochastic rounding
+  const float* lr_dev;                                // replaces lr where given
+  const float* coef;                                  // {ibc1, rbc2, key bits} where given
+};
+
+struct AdamEntry {  // m, v: float moments, or codes with their scale bytes
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  int64_t numel;
+  uint32_t word;  // dtype 0-1, vector path 2, group 3-7, place 8-31... (see entry_word)
+  uint32_t pad;
+};
+
+struct AdamEntry8 {
+  void* p;
+  const void* g;
+  uint8_t* m;
+  uint8_t* v;
+  uint8_t* ms;
+  uint8_t* vs;
+  int64_t numel;
+  uint32_t word;
+  uint32_t pad;
+};
+
+constexpr uint32_t entry_word(int dtype, bool vec, int group, int place) {
+  return (uint32_t)dtype | (vec ? 4u : 0u) | ((uint32_t)group << 3) | ((uint32_t)place << 8);
+}
+static_assert(CS_ADAMW_MAX_GROUPS <= 32, "five bits of group");
+
+template <class Entry, int N>
+struct Table {
+  int count;
+  const float* grad_scale;
+  AdamGroup groups[CS_ADAMW_MAX_GROUPS];
+  int first[N];  // first chunk of each entry
+  Entry e[N];
+};
+
+__device__ __forceinline__ int find_entry(const int* first, int count, int chunk) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= chunk)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------
+// Eight elements of a thread as float32: contiguous ones with wide accesses
+// (the pointer aligned to eight elements), or every 32nd of the warp's 256.
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+template <class T>
+struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) Pack8 {
+  T x[8];
+};
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const Pack8<T> q = *reinterpret_cast<const Pack8<T>*>(p);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) x[u] = to_f32(q.x[u]);
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  Pack8<T> q;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) q.x[u] = from_f32<T>(x[u]);
+  *reinterpret_cast<Pack8<T>*>(p) = q;
+}
+
+struct StepCoef {
+  float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale;
+  uint32_t key;
+};
+
+__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale) {
+  StepCoef c;
+  c.b1 = g.b1;
+  c.omb1 = g.omb1;
+  c.b2 = g.b2;
+  c.omb2 = g.omb2;
+  c.eps = g.eps;
+  const float lr = g.lr_dev ? __ldg(g.lr_dev) : g.lr;
+  float ibc1 = g.ibc1;
+  c.rbc2 = g.rbc2;
+  c.key = g.key;
+  if (g.coef) {
+    ibc1 = __ldg(g.coef);
+    c.rbc2 = __ldg(g.coef + 1);
+    c.key = __float_as_uint(__ldg(g.coef + 2));
+  }
+  c.step_size = lr * ibc1;
+  c.decay = __fmaf_rn(-lr, g.wd, 1.0f);
+  c.scale = grad_scale ? __ldg(grad_scale) : 1.0f;
+  return c;
+}
+
+// One element.  The moments' arithmetic is one rounding an operation in the
+// order written; the 8-bit moments' bytes are defined by it.
+__device__ __forceinline__ void adamw_element(const StepCoef& c, float& p, float g, float& m,
+                                              float& v) {
+  g = g * c.scale;
+  m = m * c.b1 + g * c.omb1;
+  v = v * c.b2 + (g * g) * c.omb2;
+  p = p * c.decay - c.step_size * (m / (sqrtf(v) * c.rbc2 + c.eps));
+}
+
+// ---------------------------------------------------------------------------
+// 32-bit moments
+
+template <class T>
+__device__ __forceinline__ void step_chunk(const AdamEntry& e, const StepCoef& c, int64_t at) {
+  T* p = static_cast<T*>(e.p) + at;
+  const T* g = static_cast<const T*>(e.g) + at;
+  float* m = static_cast<float*>(e.m) + at;
+  float* v = static_cast<float*>(e.v) + at;
+  const int lane = threadIdx.x & 31, base = (threadIdx.x >> 5) * kBlock8;
+  const int64_t left = e.numel - at - base;
+  if (left <= 0) return;
+  float P[8], G[8], M[8], V[8];
+  if ((e.word & 4) && left >= kBlock8) {
+    const int i = base + lane * 8;
+    load8(p + i, P);
+    load8(g + i, G);
+    load8(m + i, M);
+    load8(v + i, V);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) adamw_element(c, P[u], G[u], M[u], V[u]);
+    store8(p + i, P);
+    store8(m + i, M);
+    store8(v + i, V);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = base + lane + 32 * u;
+      if (lane + 32 * u < left) {
+        P[u] = to_f32(p[i]);
+        G[u] = to_f32(g[i]);
+        M[u] = m[i];
+        V[u] = v[i];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = base + lane + 32 * u;
+      if (lane + 32 * u < left) {
+        adamw_element(c, P[u], G[u], M[u], V[u]);
+        p[i] = from_f32<T>(P[u]);
+        m[i] = M[u];
+        v[i] = V[u];
+      }
+    }
+  }
+}
+
+template <int N>
+__global__ void __launch_bounds__(kChunkThreads)
+    adamw_kernel(const __grid_constant__ Table<AdamEntry, N> t) {
+  const int k = find_entry(t.first, t.count, blockIdx.x);
+  const AdamEntry& e = t.e[k];
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
+  switch (e.word & 3) {
+    case CS_F32: step_chunk<float>(e, c, at); break;
+    case CS_BF16: step_chunk<__nv_bfloat16>(e, c, at); break;
+    default: step_chunk<__half>(e, c, at); break;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit moments
+//
+// A block of 256 elements (one warp, eight a lane) shares one scale byte E that
+// stands for 2^(E-127): the smallest power of two, E >= 40, with
+// max|x| <= 1.875 * 2^(E-127).  x / 2^(E-127) is multiplied by 2^-112 (m) or
+// 2^-96 (v), which puts the largest value at the exponent field 15 (m) or 31
+// (v) of a float32, and the code is that float's bits 20..26 with the sign (m:
+// sign, 4 exponent, 3 fraction bits) or 20..27 (v: 5 and 3), the float's own
+// gradual underflow included.  Decoding is the same shift and two exact
+// multiplications, one of which is the beta of the average.  The 20 low bits
+// go by stochastic rounding: a moment that moves by 1 - beta2 = 0.1% a step
+// would never leave its code (6 to 12% wide) by rounding to nearest.  A v above
+// zero keeps at least its smallest code, so that m / sqrt(v) stays bounded.
+// E = 255 marks a block whose largest magnitude is NaN or needs E >= 254; all
+// of its elements then stand for NaN.
+
+constexpr int kMinScale = 40;
+constexpr float kTwoM112 = 1.925929944387236e-34f, kTwo112 = 5.192296858534828e33f;
+constexpr float kTwoM96 = 1.262177448353619e-29f, kTwo96 = 7.922816251426434e28f;
+
+__host__ __device__ constexpr uint32_t mix32(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x6A09E667u;
+  h = (h ^ (h >> 15)) * 0xBB67AE85u;
+  return h ^ (h >> 16);
+}
+// Key of a step, of a block of a tensor, and the 32 random bits of an element:
+// multiply-xorshift mixing with fractional digits of square roots and the
+// golden ratio as multipliers.
+__host__ __device__ constexpr uint32_t step_key(uint32_t seed, uint32_t step) {
+  return mix32(seed + step * 0x9E3779B1u);
+}
+__device__ __forceinline__ uint32_t block_key(uint32_t key, uint32_t place, uint32_t block) {
+  return mix32(key + place * 0x3C6EF373u + block * 0xA54FF53Bu);
+}
+__device__ __forceinline__ uint32_t element_bits(uint32_t block, uint32_t at) {
+  uint32_t h = block + at * 0x9E3779B1u;
+  h = (h ^ (h >> 16)) * 0x6A09E667u;
+  return h ^ (h >> 15);
+}
+
+__device__ __forceinline__ float scale_unit(uint32_t e) {
+  return e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float(e << 23);
+}
+__device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits) {
+  const uint32_t e = max((largest_bits + 0xFFFFFu) >> 23, (uint32_t)kMinScale);
+  return e >= 254 ? 255u : e;
+}
+__device__ __forceinline__ float scale_inverse(uint32_t e) {
+  return e == 255 ? 0.0f : __uint_as_float((254u - e) << 23);
+}
+__device__ __forceinline__ float decode_m(uint32_t code) {  // times 2^(E-127)
+  return __uint_as_float(((code & 127u) << 20) | ((code & 128u) << 24)) * kTwo112;
+}
+__device__ __forceinline__ float decode_v(uint32_t code) {
+  return __uint_as_float(code << 20) * kTwo96;
+}
+__device__ __forceinline__ uint32_t encode_m(float x, float inverse, uint32_t rand16) {
+  const uint32_t i = __float_as_uint((x * inverse) * kTwoM112);
+  return ((((i & 0x7fffffffu) + (rand16 << 4)) >> 20) & 127u) | ((i >> 24) & 128u);
+}
+__device__ __forceinline__ uint32_t encode_v(float x, float inverse, uint32_t rand16) {
+  const uint32_t i = __float_as_uint((x * inverse) * kTwoM96) & 0x7fffffffu;
+  return max((i + (rand16 << 4)) >> 20, x > 0.0f ? 1u : 0u) & 255u;
+}
+
+template <class T, bool kVec>
+__device__ __forceinline__ void step_block8(const AdamEntry8& e, const StepCoef& c, int64_t block,
+                                            int64_t left) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = block * kBlock8;
+  T* p = static_cast<T*>(e.p) + at;
+  const T* g = static_cast<const T*>(e.g) + at;
+  uint8_t* mc = e.m + at;
+  uint8_t* vc = e.v + at;
+  float P[8], G[8];
+  uint32_t MC[8], VC[8];
+  if (kVec) {
+    load8(p + lane * 8, P);
+    load8(g + lane * 8, G);
+    const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
+    const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      MC[u] = ((u < 4 ? a.x : a.y) >> (8 * (u & 3))) & 255u;
+      VC[u] = ((u < 4 ? b.x : b.y) >> (8 * (u & 3))) & 255u;
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = lane + 32 * u;
+      const bool in = i < left;
+      P[u] = in ? to_f32(p[i]) : 0.0f;
+      G[u] = in ? to_f32(g[i]) : 0.0f;
+      MC[u] = in ? mc[i] : 0u;
+      VC[u] = in ? vc[i] : 0u;
+    }
+  }
+  const float mb = scale_unit(e.ms[block]), vb = scale_unit(e.vs[block]);
+  float M[8], V[8];
+  uint32_t mmax = 0, vmax = 0;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const bool in = kVec || lane + 32 * u < left;
+    M[u] = decode_m(MC[u]) * mb;
+    V[u] = decode_v(VC[u]) * vb;
+    adamw_element(c, P[u], G[u], M[u], V[u]);
+    mmax = max(mmax, in ? __float_as_uint(M[u]) & 0x7fffffffu : 0u);
+    vmax = max(vmax, in ? __float_as_uint(V[u]) & 0x7fffffffu : 0u);
+  }
+  const uint32_t me = scale_byte(__reduce_max_sync(0xffffffffu, mmax));
+  const uint32_t ve = scale_byte(__reduce_max_sync(0xffffffffu, vmax));
+  const float mi = scale_inverse(me), vi = scale_inverse(ve);
+  const uint32_t key = block_key(c.key, e.word >> 8, (uint32_t)block);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const uint32_t r = element_bits(key, kVec ? lane * 8 + u : lane + 32 * u);
+    MC[u] = encode_m(M[u], mi, r & 0xFFFFu);
+    VC[u] = encode_v(V[u], vi, r >> 16);
+  }
+  if (kVec) {
+    store8(p + lane * 8, P);
+    uint2 a = make_uint2(0, 0), b = make_uint2(0, 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      a.x |= MC[u] << (8 * u);
+      a.y |= MC[u + 4] << (8 * u);
+      b.x |= VC[u] << (8 * u);
+      b.y |= VC[u + 4] << (8 * u);
+    }
+    *reinterpret_cast<uint2*>(mc + lane * 8) = a;
+    *reinterpret_cast<uint2*>(vc + lane * 8) = b;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = lane + 32 * u;
+      if (i < left) {
+        p[i] = from_f32<T>(P[u]);
+        mc[i] = (uint8_t)MC[u];
+        vc[i] = (uint8_t)VC[u];
+      }
+    }
+  }
+  if (lane == 0) {
+    e.ms[block] = (uint8_t)me;
+    e.vs[block] = (uint8_t)ve;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef& c, int64_t at) {
+  const int64_t block = at / kBlock8 + (threadIdx.x >> 5);
+  const int64_t left = e.numel - block * kBlock8;
+  if (left <= 0) return;
+  if ((e.word & 4) && left >= kBlock8)
+    step_block8<T, true>(e, c, block, left);
+  else
+    step_block8<T, false>(e, c, block, left);
+}
+
+template <int N>
+__global__ void __launch_bounds__(kChunkThreads)
+    adamw8_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
+  const int k = find_entry(t.first, t.count, blockIdx.x);
+  const AdamEntry8& e = t.e[k];
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
+  const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
+  switch (e.word & 3) {
+    case CS_F32: step_warp8<float>(e, c, at); break;
+    case CS_BF16: step_warp8<__nv_bfloat16>(e, c, at); break;
+    default: step_warp8<__half>(e, c, at); break;
+  }
+}
+
+// Values of 8-bit moments: entries hold the float outputs in p (m) and g (v).
+template <int N>
+__global__ void __launch_bounds__(kChunkThreads)
+    adamw8_moments_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
+  const int k = find_entry(t.first, t.count, blockIdx.x);
+  const AdamEntry8& e = t.e[k];
+  const int lane = threadIdx.x & 31;
+  const int64_t block =
+      (int64_t)((int)blockIdx.x - t.first[k]) * (kChunk / kBlock8) + (threadIdx.x >> 5);
+  const int64_t left = e.numel - block * kBlock8;
+  if (left <= 0) return;
+  float* om = static_cast<float*>(e.p) + block * kBlock8;
+  float* ov = static_cast<float*>(const_cast<void*>(e.g)) + block * kBlock8;
+  const uint8_t* mc = e.m + block * kBlock8;
+  const uint8_t* vc = e.v + block * kBlock8;
+  const float mb = scale_unit(e.ms[block]), vb = scale_unit(e.vs[block]);
+  if ((e.word & 4) && left >= kBlock8) {
+    const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
+    const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
+    float M[8], V[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      M[u] = decode_m(((u < 4 ? a.x : a.y) >> (8 * (u & 3))) & 255u) * mb;
+      V[u] = decode_v(((u < 4 ? b.x : b.y) >> (8 * (u & 3))) & 255u) * vb;
+    }
+    store8(om + lane * 8, M);
+    store8(ov + lane * 8, V);
+  } else {
+    for (int i = lane; i < kBlock8 && i < left; i += 32) {
+      om[i] = decode_m(mc[i]) * mb;
+      ov[i] = decode_v(vc[i]) * vb;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Bias corrections and rounding keys from device step counters: thread i
+// advances group i's counter and writes {1/(1-b1^t), 1/sqrt(1-b2^t), key}.
+struct AdvanceArgs {
+  int count;
+  uint32_t seed;
+  float* coef;
+  int64_t* step[CS_ADAMW_MAX_GROUPS];
+  double b1[CS_ADAMW_MAX_GROUPS], b2[CS_ADAMW_MAX_GROUPS];
+};
+
+__global__ void adamw_advance_kernel(const __grid_constant__ AdvanceArgs a) {
+  const int i = threadIdx.x;
+  if (i >= a.count) return;
+  const int64_t t = *a.step[i] + 1;
+  *a.step[i] = t;
+  a.coef[4 * i] = (float)(1.0 / (1.0 - pow(a.b1[i], (double)t)));
+  a.coef[4 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2[i], (double)t)));
+  a.coef[4 * i + 2] = __uint_as_float(step_key(a.seed, (uint32_t)t));
+}
+
+// ---------------------------------------------------------------------------
+// Global gradient norm: per-CTA sums in double in a fixed order, then one CTA.
+// Squares are formed in double, so neither 1e30 nor 1e-30 is lost.
+
+struct NormEntry {
+  const void* g;
+  int64_t numel;
+};
+
+template <int N>
+struct NormTable {
+  int count, chunks;
+  double* partials;
+  int first[N];
+  uint8_t word[N];
+  NormEntry e[N];
+};
+
+constexpr int kNormThreads = 256;
+constexpr int kNormChunk = kNormThreads * 32;
+constexpr int kNormBlocks = 148 * 4;
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ double block_sum_d(double v) {  // valid in thread 0
+  __shared__ double sh[32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  v = warp_sum_d(v);
+  if (lane == 0) sh[wid] = v;
+  __syncthreads();
+  double r = 0.0;
+  if (wid == 0) {
+    r = lane < (int)(blockDim.x >> 5) ? sh[lane] : 0.0;
+    r = warp_sum_d(r);
+  }
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ double norm_chunk(const void* data, int64_t at, int64_t numel,
+                                             bool vec) {
+  const T* g = static_cast<const T*>(data) + at;
+  const int64_t left = numel - at;
+  const int n = left < kNormChunk ? (int)left : kNormChunk;
+  double acc = 0.0;
+  if (vec) {
+    float x[4][8];
+    if (n == kNormChunk) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load8(g + (u * kNormThreads + threadIdx.x) * 8, x[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc = fma((double)x[u][j], (double)x[u][j], acc);
+      return acc;
+    }
+    for (int i = threadIdx.x * 8; i + 8 <= n; i += kNormThreads * 8) {
+      load8(g + i, x[0]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc = fma((double)x[0][j], (double)x[0][j], acc);
+    }
+    for (int i = (n & ~7) + threadIdx.x; i < n; i += kNormThreads) {
+      const double y = to_f32(g[i]);
+      acc = fma(y, y, acc);
+    }
+    return acc;
+  }
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += kNormThreads) {
+    const double y = to_f32(g[i]);
+    acc = fma(y, y, acc);
+  }
+  return acc;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kNormThreads)
+    grad_norm_kernel(const __grid_constant__ NormTable<N> t) {
+  double acc = 0.0;
+  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+    const int k = find_entry(t.first, t.count, c);
+    const NormEntry& e = t.e[k];
+    const int64_t at = (int64_t)(c - t.first[k]) * kNormChunk;
+    const bool vec = (t.word[k] & 4) != 0;
+    switch (t.word[k] & 3) {
+      case CS_F32: acc += norm_chunk<float>(e.g, at, e.numel, vec); break;
+      case CS_BF16: acc += norm_chunk<__nv_bfloat16>(e.g, at, e.numel, vec); break;
+      default: acc += norm_chunk<__half>(e.g, at, e.numel, vec); break;
+    }
+  }
+  acc = block_sum_d(acc);
+  if (threadIdx.x == 0) t.partials[blockIdx.x] = acc;
+}
+
+__global__ void __launch_bounds__(256)
+    grad_norm_finish_kernel(const double* __restrict__ partials, int n, double max_norm,
+                            double eps, float* __restrict__ norm, float* __restrict__ scale) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) acc += partials[i];
+  acc = block_sum_d(acc);
+  if (threadIdx.x == 0) {
+    const double r = sqrt(acc);
+    *norm = (float)r;
+    if (scale) {
+      const double q = max_norm / (r + eps);
+      *scale = max_norm > 0.0 ? (q > 1.0 ? 1.0f : (float)q) : 1.0f;  // NaN stays NaN
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+
+inline int dtype_size(int d) { return d == CS_F32 ? 4 : 2; }
+inline bool aligned_to(const void* q, int bytes) {
+  return (reinterpret_cast<uintptr_t>(q) & (uintptr_t)(bytes - 1)) == 0;
+}
+
+struct GroupBuilder {
+  AdamGroup g[CS_ADAMW_MAX_GROUPS];
+  int fill(const cs_adamw_group* groups, int n, const float* coef, uint32_t seed) {
+    for (int i = 0; i < n; ++i) {
+      const cs_adamw_group& s = groups[i];
+      if (!(s.beta1 >= 0.0 && s.beta1 < 1.0 && s.beta2 >= 0.0 && s.beta2 < 1.0)) return CS_ERR_ARG;
+      if (!coef && s.step < 1) return CS_ERR_ARG;
+      AdamGroup& d = g[i];
+      d.b1 = (float)s.beta1;
+      d.omb1 = (float)(1.0 - s.beta1);
+      d.b2 = (float)s.beta2;
+      d.omb2 = (float)(1.0 - s.beta2);
+      d.eps = (float)s.eps;
+      d.lr = (float)s.lr;
+      d.wd = (float)s.weight_decay;
+      d.lr_dev = s.lr_device;
+      d.coef = coef ? coef + 4 * i : nullptr;
+      d.ibc1 = d.rbc2 = 0.0f;
+      d.key = 0;
+      if (!coef) {
+        d.ibc1 = (float)(1.0 / (1.0 - std::pow(s.beta1, (double)s.step)));
+        d.rbc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(s.beta2, (double)s.step)));
+        d.key = step_key(seed, (uint32_t)s.step);
+      }
+    }
+    for (int i = n; i < CS_ADAMW_MAX_GROUPS; ++i) g[i] = AdamGroup{};
+    return CS_OK;
+  }
+};
+
+inline bool make_entry(const cs_adamw_tensor& s, int place, AdamEntry& e) {
+  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq) return false;
+  const int w = 8 * dtype_size(s.dtype) < 16 ? 8 * dtype_size(s.dtype) : 16;
+  const bool vec = aligned_to(s.param, w) && aligned_to(s.grad, w) && aligned_to(s.exp_avg, 16) &&
+                   aligned_to(s.exp_avg_sq, 16);
+  e = AdamEntry{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.numel,
+                entry_word(s.dtype, vec, s.group, place), 0};
+  return true;
+}
+
+inline bool make_entry(const cs_adamw_tensor& s, int place, AdamEntry8& e) {
+  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !s.exp_avg_scales ||
+      !s.exp_avg_sq_scales)
+    return false;
+  const bool vec = aligned_to(s.param, 16) && aligned_to(s.grad, 16) && aligned_to(s.exp_avg, 8) &&
+                   aligned_to(s.exp_avg_sq, 8);
+  e = AdamEntry8{s.param,
+                 s.grad,
+                 static_cast<uint8_t*>(s.exp_avg),
+                 static_cast<uint8_t*>(s.exp_avg_sq),
+                 s.exp_avg_scales,
+                 s.exp_avg_sq_scales,
+                 s.numel,
+                 entry_word(s.dtype, vec, s.group, place),
+                 0};
+  return true;
+}
+
+// The kernels of one table type, by name.
+struct RunStep {
+  template <int N>
+  static void launch(const Table<AdamEntry, N>& t, int chunks, cudaStream_t st) {
+    adamw_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
+  }
+};
+struct RunStep8 {
+  template <int N>
+  static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
+    adamw8_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
+  }
+};
+struct RunMoments8 {
+  template <int N>
+  static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
+    adamw8_moments_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
+  }
+};
+
+// Packs tensors (empty ones left out) into tables of at most N entries and
+// launches each full one.
+template <class Run, class Entry, int N>
+int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const AdamGroup* g,
+                  const float* grad_scale, cudaStream_t st) {
+  Table<Entry, N> t;
+  t.grad_scale = grad_scale;
+  for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
+  t.count = 0;
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) {
+    const cs_adamw_tensor& s = tensors[i];
+    if (s.numel == 0) continue;
+    const int64_t mine = (s.numel + kChunk - 1) / kChunk;
+    if (t.count == N || chunks + mine > INT32_MAX) {
+      Run::template launch<N>(t, (int)chunks, st);
+      if (int rc = launch_status()) return rc;
+      t.count = 0;
+      chunks = 0;
+    }
+    if (!make_entry(s, i, t.e[t.count])) return CS_ERR_ARG;
+    t.first[t.count++] = (int)chunks;
+    chunks += mine;
+  }
+  if (t.count == 0) return CS_OK;
+  Run::template launch<N>(t, (int)chunks, st);
+  return launch_status();
+}
+
+inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups) {
+  if (count < 0 || count > kMaxTensors || (count > 0 && !tensors)) return CS_ERR_ARG;
+  for (int i = 0; i < count; ++i) {
+    const cs_adamw_tensor& s = tensors[i];
+    if (s.numel < 0 || s.numel > kMaxNumel || s.dtype < CS_F32 || s.dtype > CS_F16 ||
+        s.group < 0 || s.group >= groups)
+      return CS_ERR_ARG;
+  }
+  return CS_OK;
+}
+
+// A call of few tensors takes a small table (its parameters stay below 4 KB).
+template <class Run, class Entry, int kSmall, int kLarge>
+int run_tables(const cs_adamw_tensor* tensors, int count, int groups, const AdamGroup* g,
+               const float* grad_scale, cudaStream_t st) {
+  static_assert(sizeof(Table<Entry, kLarge>) <= 32764, "kernel parameter limit");
+  if (count <= kSmall)
+    return launch_tables<Run, Entry, kSmall>(tensors, count, groups, g, grad_scale, st);
+  return launch_tables<Run, Entry, kLarge>(tensors, count, groups, g, grad_scale, st);
+}
+
+template <class Run, class Entry, int kSmall, int kLarge>
+int step_entry(const cs_adamw_tensor* tensors, int count, const cs_adamw_group* groups,
+               int num_groups, const float* coef, uint32_t seed, const float* grad_scale,
+               void* stream) {
+  if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups) return CS_ERR_ARG;
+  if (int rc = check_tensors(tensors, count, num_groups)) return rc;
+  GroupBuilder b;
+  if (int rc = b.fill(groups, num_groups, coef, seed)) return rc;
+  return run_tables<Run, Entry, kSmall, kLarge>(tensors, count, num_groups, b.g, grad_scale,
+                                                (cudaStream_t)stream);
+}
+
+template <int N>
+int launch_norm(const cs_grad_tensor* tensors, int count, double* partials, int& used, int room,
+                cudaStream_t st) {
+  NormTable<N> t;
+  t.count = 0;
+  int64_t chunks = 0;
+  auto flush = [&]() {
+    t.chunks = (int)chunks;
+    const int blocks = chunks < kNormBlocks ? (int)chunks : kNormBlocks;
+    if (used + blocks > room) return (int)CS_ERR_CAPACITY;
+    t.partials = partials + used;
+    grad_norm_kernel<N><<<blocks, kNormThreads, 0, st>>>(t);
+    used += blocks;
+    t.count = 0;
+    chunks = 0;
+    return launch_status();
+  };
+  for (int i = 0; i < count; ++i) {
+    const cs_grad_tensor& s = tensors[i];
+    if (s.numel == 0) continue;
+    const int64_t mine = (s.numel + kNormChunk - 1) / kNormChunk;
+    if (t.count == N || chunks + mine > INT32_MAX - kNormBlocks)
+      if (int rc = flush()) return rc;
+    t.e[t.count] = NormEntry{s.data, s.numel};
+    t.word[t.count] = (uint8_t)(s.dtype | (aligned_to(s.data, 16) ? 4 : 0));
+    t.first[t.count++] = (int)chunks;
+    chunks += mine;
+  }
+  return t.count ? flush() : (int)CS_OK;
+}
+
+constexpr int kNormSmall = 128, kNormLarge = 1400;
+static_assert(sizeof(NormTable<kNormLarge>) <= 32764, "kernel parameter limit");
+
+}  // namespace cs
+
+using namespace cs;
+
+extern "C" {
+
+int cs_adamw_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
+                  int32_t num_groups, const float* coef, const float* grad_scale, void* stream) {
+  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, coef, 0,
+                                                 grad_scale, stream);
+}
+
+int cs_adamw8_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
+                   int32_t num_groups, const float* coef, uint32_t seed, const float* grad_scale,
+                   void* stream) {
+  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, coef, seed,
+                                                   grad_scale, stream);
+}
+
+int cs_adamw8_moments(const cs_adamw_tensor* tensors, int32_t count, void* stream) {
+  if (int rc = check_tensors(tensors, count, 1)) return rc;
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].dtype != CS_F32) return CS_ERR_ARG;
+  return run_tables<RunMoments8, AdamEntry8, 36, 420>(tensors, count, 1, nullptr, nullptr,
+                                                      (cudaStream_t)stream);
+}
+
+int cs_adamw_advance(int64_t* const* steps, const cs_adamw_group* groups, int32_t num_groups,
+                     uint32_t seed, float* coef, void* stream) {
+  if (!steps || !groups || !coef || num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS)
+    return CS_ERR_ARG;
+  AdvanceArgs a{};
+  a.count = num_groups;
+  a.seed = seed;
+  a.coef = coef;
+  for (int i = 0; i < num_groups; ++i) {
+    if (!steps[i]) return CS_ERR_ARG;
+    for (int j = 0; j < i; ++j)
+      if (steps[j] == steps[i]) return CS_ERR_ARG;  // each counter advances once
+    a.step[i] = steps[i];
+    a.b1[i] = groups[i].beta1;
+    a.b2[i] = groups[i].beta2;
+  }
+  adamw_advance_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(a);
+  return launch_status();
+}
+
+size_t cs_grad_norm_workspace_size(int32_t count) {
+  const size_t launches = count <= 0 ? 1 : ((size_t)count + kNormSmall - 1) / kNormSmall + 1;
+  return launches * kNormBlocks * sizeof(double);
+}
+
+int cs_grad_norm(const cs_grad_tensor* tensors, int32_t count, double max_norm, double eps,
+                 float* norm, float* scale, void* workspace, void* stream) {
+  if (count < 0 || count > kMaxTensors || (count > 0 && !tensors) || !norm || !workspace ||
+      !aligned_to(workspace, 8))
+    return CS_ERR_ARG;
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || tensors[i].dtype < CS_F32 ||
+        tensors[i].dtype > CS_F16 || (tensors[i].numel > 0 && !tensors[i].data))
+      return CS_ERR_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  double* partials = static_cast<double*>(workspace);
+  const int room = (int)(cs_grad_norm_workspace_size(count) / sizeof(double));
+  int used = 0;
+  const int rc = count <= kNormSmall
+                     ? launch_norm<kNormSmall>(tensors, count, partials, used, room, st)
+                     : launch_norm<kNormLarge>(tensors, count, partials, used, room, st);
+  if (rc) return rc;
+  grad_norm_finish_kernel<<<1, 256, 0, st>>>(partials, used, max_norm, eps, norm, scale);
+  return launch_status();
+}
+
+}  // extern "C"

@@ -699,6 +699,8 @@ void forget_capacities() {
   g_caps.clear();
 }
 
+void bind_adamw(py::module_& m);  // torch_adamw.cpp
+
 PYBIND11_MODULE(_cs_torch, m) {
   m.doc() = "torch binding of the B200 CubicSplat C ABI (one call per autograd stage)";
   py::class_<Frame, FrameP>(m, "Frame")
@@ -755,4 +757,5 @@ PYBIND11_MODULE(_cs_torch, m) {
   m.def("mse_backward", &mse_backward);
   m.def("ssim_planes", &ssim_planes);
   m.def("forget_capacities", &forget_capacities);
+  bind_adamw(m);
 }
