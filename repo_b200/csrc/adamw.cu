@@ -67,6 +67,7 @@ static_assert(CS_ADAMW_MAX_GROUPS <= 32, "five bits of group");
 template <class Entry, int N>
 struct Table {
   int count;
+  float one;  // 1 (see sum2)
   const float* grad_scale;
   AdamGroup groups[CS_ADAMW_MAX_GROUPS];
   int first[N];  // first chunk of each entry
@@ -122,13 +123,40 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<Pack8<T>*>(p) = q;
 }
 
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float2 (&x)[4]) {
+  const Pack8<T> q = *reinterpret_cast<const Pack8<T>*>(p);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) x[u] = make_float2(to_f32(q.x[2 * u]), to_f32(q.x[2 * u + 1]));
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float2 (&x)[4]) {
+  Pack8<T> q;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    q.x[2 * u] = from_f32<T>(x[u].x);
+    q.x[2 * u + 1] = from_f32<T>(x[u].y);
+  }
+  *reinterpret_cast<Pack8<T>*>(p) = q;
+}
+
+// One 32-byte store of a lane (aligned to 32 bytes): whole sectors at once.
+__device__ __forceinline__ void store_wide(float* p, const float2 (&x)[4]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0].x),
+               "f"(x[0].y), "f"(x[1].x), "f"(x[1].y), "f"(x[2].x), "f"(x[2].y), "f"(x[3].x),
+               "f"(x[3].y)
+               : "memory");
+}
+
 struct StepCoef {
-  float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale;
+  float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale, one;
   uint32_t key;
 };
 
-__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale) {
+__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale,
+                                            float one) {
   StepCoef c;
+  c.one = one;
   c.b1 = g.b1;
   c.omb1 = g.omb1;
   c.b2 = g.b2;
@@ -212,7 +240,7 @@ __global__ void __launch_bounds__(kChunkThreads)
     adamw_kernel(const __grid_constant__ Table<AdamEntry, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
   switch (e.word & 3) {
     case CS_F32: step_chunk<float>(e, c, at); break;
@@ -249,24 +277,18 @@ __host__ __device__ constexpr uint32_t mix32(uint32_t h) {
 }
 // Key of a step, of a block of a tensor, and the 32 random bits of an element:
 // multiply-xorshift mixing with fractional digits of square roots and the
-// golden ratio as multipliers.
+// golden ratio as multipliers (an element's bits in step_lane8).
 __host__ __device__ constexpr uint32_t step_key(uint32_t seed, uint32_t step) {
   return mix32(seed + step * 0x9E3779B1u);
 }
 __device__ __forceinline__ uint32_t block_key(uint32_t key, uint32_t place, uint32_t block) {
   return mix32(key + place * 0x3C6EF373u + block * 0xA54FF53Bu);
 }
-__device__ __forceinline__ uint32_t element_bits(uint32_t block, uint32_t at) {
-  uint32_t h = block + at * 0x9E3779B1u;
-  h = (h ^ (h >> 16)) * 0x6A09E667u;
-  return h ^ (h >> 15);
-}
-
 __device__ __forceinline__ float scale_unit(uint32_t e) {
   return e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float(e << 23);
 }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits) {
-  const uint32_t e = max((largest_bits + 0xFFFFFu) >> 23, (uint32_t)kMinScale);
+  const uint32_t e = max((largest_bits + 0xFFFFFu) >> 23, (uint32_t)kMinScale);  // NaN: 256
   return e >= 254 ? 255u : e;
 }
 __device__ __forceinline__ float scale_inverse(uint32_t e) {
@@ -278,13 +300,129 @@ __device__ __forceinline__ float decode_m(uint32_t code) {  // times 2^(E-127)
 __device__ __forceinline__ float decode_v(uint32_t code) {
   return __uint_as_float(code << 20) * kTwo96;
 }
-__device__ __forceinline__ uint32_t encode_m(float x, float inverse, uint32_t rand16) {
-  const uint32_t i = __float_as_uint((x * inverse) * kTwoM112);
-  return ((((i & 0x7fffffffu) + (rand16 << 4)) >> 20) & 127u) | ((i >> 24) & 128u);
+
+// x + y of pairs, one rounding each.  A packed sum of a packed product is fused
+// by the assembler whatever rounding both are written with, which would round
+// once instead of twice; as x * one + y with a `one` that only the host knows it
+// is the same sum and cannot be.
+__device__ __forceinline__ float2 sum2(float2 x, float2 one, float2 y) {
+  return __ffma2_rn(x, one, y);
 }
-__device__ __forceinline__ uint32_t encode_v(float x, float inverse, uint32_t rand16) {
-  const uint32_t i = __float_as_uint((x * inverse) * kTwoM96) & 0x7fffffffu;
-  return max((i + (rand16 << 4)) >> 20, x > 0.0f ? 1u : 0u) & 255u;
+__device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 bits2(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+// max(|a|, |b|, |c|), NaN if any is
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Codes u and u+1 of a word of four, as the float2 whose bits they are.
+template <int U>
+__device__ __forceinline__ float2 bits_m(uint32_t w) {
+  // the code in the top byte: its sign is the float's, its magnitude 4 down
+  const int a = (int)(w << (24 - 8 * U)), b = (int)(w << (16 - 8 * U));
+  return bits2((uint32_t)(a >> 4) & 0x87F00000u, (uint32_t)(b >> 4) & 0x87F00000u);
+}
+template <int U>
+__device__ __forceinline__ float2 bits_v(uint32_t w) {
+  return bits2((w << (20 - 8 * U)) & 0x0FF00000u,
+               (U == 0 ? w << 12 : w >> 4) & 0x0FF00000u);
+}
+// The two 16-bit tops of a pair of floats' bits in one word.
+__device__ __forceinline__ uint32_t tops(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x7632);
+}
+
+// A lane's eight elements of one block: P and the codes in mw, vw in, the same
+// out, and the block's new scale bytes.  Arithmetic on m and v is in float32
+// pairs (two independent IEEE operations an instruction) in the written order;
+// decoding's power of two is folded into beta, which changes no bit.  The
+// parameter's update uses the hardware's square root and reciprocal, each
+// within 2^-22: the bytes do not depend on it.
+// `first` is the element of the lane's first value in the block, `stride` the
+// distance of the next.
+template <int kStride>
+__device__ __forceinline__ void step_lane8(const StepCoef& c, float2 (&P)[4], float2 (&G)[4],
+                                           uint32_t (&mw)[2], uint32_t (&vw)[2], float mb,
+                                           float vb, uint32_t key, uint32_t first, uint32_t& me,
+                                           uint32_t& ve) {
+  const float2 scale = pair(c.scale), omb1 = pair(c.omb1), omb2 = pair(c.omb2), one = pair(c.one);
+  const float2 mk = pair(c.b1 * mb), vk = pair(c.b2 * vb);
+  const float2 up112 = pair(kTwo112), up96 = pair(kTwo96);
+  float2 M[4], V[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    M[u] = (u & 1) ? bits_m<2>(mw[u >> 1]) : bits_m<0>(mw[u >> 1]);
+    V[u] = (u & 1) ? bits_v<2>(vw[u >> 1]) : bits_v<0>(vw[u >> 1]);
+  }
+  float mmax = 0.0f, vmax = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float2 g = __fmul2_rn(G[u], scale);
+    M[u] = sum2(__fmul2_rn(__fmul2_rn(M[u], up112), mk), one, __fmul2_rn(g, omb1));
+    V[u] = sum2(__fmul2_rn(__fmul2_rn(V[u], up96), vk), one,
+                __fmul2_rn(__fmul2_rn(g, g), omb2));
+    mmax = max3_abs(mmax, M[u].x, M[u].y);
+    vmax = max3_abs(vmax, V[u].x, V[u].y);
+    // v below the smallest normal number counts as that, so that its flushed
+    // root cannot leave a denominator of zero
+    const float2 root = make_float2(sqrt_approx(max_nan(V[u].x, 1.17549435e-38f)),
+                                    sqrt_approx(max_nan(V[u].y, 1.17549435e-38f)));
+    const float2 d = __ffma2_rn(root, pair(c.rbc2), pair(c.eps));
+    const float2 q = __fmul2_rn(M[u], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+    P[u] = __ffma2_rn(q, pair(-c.step_size), __fmul2_rn(P[u], pair(c.decay)));
+  }
+  me = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
+  ve = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
+  const float2 mi = pair(scale_inverse(me)), vi = pair(scale_inverse(ve));
+  const float2 down112 = pair(kTwoM112), down96 = pair(kTwoM96);
+  const uint32_t start = key + first * 0x9E3779B1u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t t[4], w[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int u = 2 * h + j;
+      const float2 ym = __fmul2_rn(__fmul2_rn(M[u], mi), down112);
+      const float2 yv = __fmul2_rn(__fmul2_rn(V[u], vi), down96);
+      uint32_t r0 = start + (uint32_t)(2 * u * kStride) * 0x9E3779B1u;
+      uint32_t r1 = start + (uint32_t)((2 * u + 1) * kStride) * 0x9E3779B1u;
+      r0 = (r0 ^ (r0 >> 16)) * 0x6A09E667u;
+      r1 = (r1 ^ (r1 >> 16)) * 0x6A09E667u;
+      r0 ^= r0 >> 15;
+      r1 ^= r1 >> 15;
+      t[2 * j] = __float_as_uint(ym.x) + ((r0 & 0xFFFFu) << 4);
+      t[2 * j + 1] = __float_as_uint(ym.y) + ((r1 & 0xFFFFu) << 4);
+      w[2 * j] = __float_as_uint(yv.x) + ((r0 >> 16) << 4);
+      w[2 * j + 1] = __float_as_uint(yv.y) + ((r1 >> 16) << 4);
+      if (V[u].x > 0.0f) w[2 * j] = max(w[2 * j], 1u << 20);
+      if (V[u].y > 0.0f) w[2 * j + 1] = max(w[2 * j + 1], 1u << 20);
+    }
+    // code = bits 20..26 (27) of each: shifted to bytes 0 and 2 of a pair's word
+    const uint32_t size = __byte_perm(tops(t[0], t[1]) >> 4, tops(t[2], t[3]) >> 4, 0x6420);
+    const uint32_t top = __byte_perm(__byte_perm(t[0], t[1], 0x0073),
+                                     __byte_perm(t[2], t[3], 0x0073), 0x5410);
+    mw[h] = (size & 0x7F7F7F7Fu) | (top & 0x80808080u);
+    vw[h] = __byte_perm(tops(w[0], w[1]) >> 4, tops(w[2], w[3]) >> 4, 0x6420);
+  }
 }
 
 template <class T, bool kVec>
@@ -296,71 +434,44 @@ __device__ __forceinline__ void step_block8(const AdamEntry8& e, const StepCoef&
   const T* g = static_cast<const T*>(e.g) + at;
   uint8_t* mc = e.m + at;
   uint8_t* vc = e.v + at;
-  float P[8], G[8];
-  uint32_t MC[8], VC[8];
+  float2 P[4], G[4];
+  uint32_t mw[2] = {0, 0}, vw[2] = {0, 0};
   if (kVec) {
     load8(p + lane * 8, P);
     load8(g + lane * 8, G);
     const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
     const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      MC[u] = ((u < 4 ? a.x : a.y) >> (8 * (u & 3))) & 255u;
-      VC[u] = ((u < 4 ? b.x : b.y) >> (8 * (u & 3))) & 255u;
-    }
+    mw[0] = a.x;
+    mw[1] = a.y;
+    vw[0] = b.x;
+    vw[1] = b.y;
   } else {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = lane + 32 * u;
       const bool in = i < left;
-      P[u] = in ? to_f32(p[i]) : 0.0f;
-      G[u] = in ? to_f32(g[i]) : 0.0f;
-      MC[u] = in ? mc[i] : 0u;
-      VC[u] = in ? vc[i] : 0u;
+      (u & 1 ? P[u >> 1].y : P[u >> 1].x) = in ? to_f32(p[i]) : 0.0f;
+      (u & 1 ? G[u >> 1].y : G[u >> 1].x) = in ? to_f32(g[i]) : 0.0f;
+      mw[u >> 2] |= (in ? (uint32_t)mc[i] : 0u) << (8 * (u & 3));
+      vw[u >> 2] |= (in ? (uint32_t)vc[i] : 0u) << (8 * (u & 3));
     }
   }
   const float mb = scale_unit(e.ms[block]), vb = scale_unit(e.vs[block]);
-  float M[8], V[8];
-  uint32_t mmax = 0, vmax = 0;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const bool in = kVec || lane + 32 * u < left;
-    M[u] = decode_m(MC[u]) * mb;
-    V[u] = decode_v(VC[u]) * vb;
-    adamw_element(c, P[u], G[u], M[u], V[u]);
-    mmax = max(mmax, in ? __float_as_uint(M[u]) & 0x7fffffffu : 0u);
-    vmax = max(vmax, in ? __float_as_uint(V[u]) & 0x7fffffffu : 0u);
-  }
-  const uint32_t me = scale_byte(__reduce_max_sync(0xffffffffu, mmax));
-  const uint32_t ve = scale_byte(__reduce_max_sync(0xffffffffu, vmax));
-  const float mi = scale_inverse(me), vi = scale_inverse(ve);
   const uint32_t key = block_key(c.key, e.word >> 8, (uint32_t)block);
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const uint32_t r = element_bits(key, kVec ? lane * 8 + u : lane + 32 * u);
-    MC[u] = encode_m(M[u], mi, r & 0xFFFFu);
-    VC[u] = encode_v(V[u], vi, r >> 16);
-  }
+  uint32_t me, ve;
+  step_lane8<kVec ? 1 : 32>(c, P, G, mw, vw, mb, vb, key, kVec ? lane * 8 : lane, me, ve);
   if (kVec) {
     store8(p + lane * 8, P);
-    uint2 a = make_uint2(0, 0), b = make_uint2(0, 0);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      a.x |= MC[u] << (8 * u);
-      a.y |= MC[u + 4] << (8 * u);
-      b.x |= VC[u] << (8 * u);
-      b.y |= VC[u + 4] << (8 * u);
-    }
-    *reinterpret_cast<uint2*>(mc + lane * 8) = a;
-    *reinterpret_cast<uint2*>(vc + lane * 8) = b;
+    *reinterpret_cast<uint2*>(mc + lane * 8) = make_uint2(mw[0], mw[1]);
+    *reinterpret_cast<uint2*>(vc + lane * 8) = make_uint2(vw[0], vw[1]);
   } else {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = lane + 32 * u;
       if (i < left) {
-        p[i] = from_f32<T>(P[u]);
-        mc[i] = (uint8_t)MC[u];
-        vc[i] = (uint8_t)VC[u];
+        p[i] = from_f32<T>(u & 1 ? P[u >> 1].y : P[u >> 1].x);
+        mc[i] = (uint8_t)(mw[u >> 2] >> (8 * (u & 3)));
+        vc[i] = (uint8_t)(vw[u >> 2] >> (8 * (u & 3)));
       }
     }
   }
@@ -386,7 +497,7 @@ __global__ void __launch_bounds__(kChunkThreads)
     adamw8_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
   switch (e.word & 3) {
     case CS_F32: step_warp8<float>(e, c, at); break;
@@ -414,14 +525,16 @@ __global__ void __launch_bounds__(kChunkThreads)
   if ((e.word & 4) && left >= kBlock8) {
     const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
     const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
-    float M[8], V[8];
+    const float2 mk = pair(mb), vk = pair(vb), up112 = pair(kTwo112), up96 = pair(kTwo96);
+    float2 M[4] = {bits_m<0>(a.x), bits_m<2>(a.x), bits_m<0>(a.y), bits_m<2>(a.y)};
+    float2 V[4] = {bits_v<0>(b.x), bits_v<2>(b.x), bits_v<0>(b.y), bits_v<2>(b.y)};
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      M[u] = decode_m(((u < 4 ? a.x : a.y) >> (8 * (u & 3))) & 255u) * mb;
-      V[u] = decode_v(((u < 4 ? b.x : b.y) >> (8 * (u & 3))) & 255u) * vb;
+    for (int u = 0; u < 4; ++u) {
+      M[u] = __fmul2_rn(__fmul2_rn(M[u], up112), mk);
+      V[u] = __fmul2_rn(__fmul2_rn(V[u], up96), vk);
     }
-    store8(om + lane * 8, M);
-    store8(ov + lane * 8, V);
+    store_wide(om + lane * 8, M);
+    store_wide(ov + lane * 8, V);
   } else {
     for (int i = lane; i < kBlock8 && i < left; i += 32) {
       om[i] = decode_m(mc[i]) * mb;
@@ -603,22 +716,23 @@ struct GroupBuilder {
   }
 };
 
-inline bool make_entry(const cs_adamw_tensor& s, int place, AdamEntry& e) {
+// The vector path needs parameters and gradients (in cs_adamw8_moments the
+// outputs) aligned to `width` bytes.
+inline bool make_entry(const cs_adamw_tensor& s, int place, int width, AdamEntry& e) {
   if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq) return false;
-  const int w = 8 * dtype_size(s.dtype) < 16 ? 8 * dtype_size(s.dtype) : 16;
-  const bool vec = aligned_to(s.param, w) && aligned_to(s.grad, w) && aligned_to(s.exp_avg, 16) &&
-                   aligned_to(s.exp_avg_sq, 16);
+  const bool vec = aligned_to(s.param, width) && aligned_to(s.grad, width) &&
+                   aligned_to(s.exp_avg, 16) && aligned_to(s.exp_avg_sq, 16);
   e = AdamEntry{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.numel,
                 entry_word(s.dtype, vec, s.group, place), 0};
   return true;
 }
 
-inline bool make_entry(const cs_adamw_tensor& s, int place, AdamEntry8& e) {
+inline bool make_entry(const cs_adamw_tensor& s, int place, int width, AdamEntry8& e) {
   if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !s.exp_avg_scales ||
       !s.exp_avg_sq_scales)
     return false;
-  const bool vec = aligned_to(s.param, 16) && aligned_to(s.grad, 16) && aligned_to(s.exp_avg, 8) &&
-                   aligned_to(s.exp_avg_sq, 8);
+  const bool vec = aligned_to(s.param, width) && aligned_to(s.grad, width) &&
+                   aligned_to(s.exp_avg, 8) && aligned_to(s.exp_avg_sq, 8);
   e = AdamEntry8{s.param,
                  s.grad,
                  static_cast<uint8_t*>(s.exp_avg),
@@ -633,18 +747,21 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, AdamEntry8& e) {
 
 // The kernels of one table type, by name.
 struct RunStep {
+  static constexpr int kWidth = 16;
   template <int N>
   static void launch(const Table<AdamEntry, N>& t, int chunks, cudaStream_t st) {
     adamw_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunStep8 {
+  static constexpr int kWidth = 16;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunMoments8 {
+  static constexpr int kWidth = 32;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_moments_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
@@ -657,6 +774,7 @@ template <class Run, class Entry, int N>
 int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const AdamGroup* g,
                   const float* grad_scale, cudaStream_t st) {
   Table<Entry, N> t;
+  t.one = 1.0f;
   t.grad_scale = grad_scale;
   for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
   t.count = 0;
@@ -671,7 +789,7 @@ int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const A
       t.count = 0;
       chunks = 0;
     }
-    if (!make_entry(s, i, t.e[t.count])) return CS_ERR_ARG;
+    if (!make_entry(s, i, Run::kWidth, t.e[t.count])) return CS_ERR_ARG;
     t.first[t.count++] = (int)chunks;
     chunks += mine;
   }
