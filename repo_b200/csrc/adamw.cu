@@ -24,7 +24,8 @@ constexpr int kPerThread = 8;
 constexpr int kBlock8 = CS_ADAMW8_BLOCK;                  // elements of a scale block: one warp's
 constexpr int kChunk = kChunkThreads * kPerThread;        // elements of a CTA's chunk
 static_assert(kBlock8 == 32 * kPerThread, "a warp holds one scale block");
-constexpr int64_t kMaxNumel = int64_t(1) << 40;
+constexpr int64_t kMaxNumel = int64_t(1) << 38;           // its scale blocks fit 32 bits
+constexpr int64_t kMaxEntry = int64_t(1) << 30;           // longer tensors take several entries
 constexpr int kMaxTensors = 1 << 22;                      // places that fit an entry's word
 
 // ---------------------------------------------------------------------------
@@ -56,7 +57,7 @@ struct AdamEntry8 {
   uint8_t* vs;
   int64_t numel;
   uint32_t word;
-  uint32_t pad;
+  uint32_t block0;  // number of its first block in its tensor
 };
 
 constexpr uint32_t entry_word(int dtype, bool vec, int group, int place) {
@@ -67,6 +68,7 @@ static_assert(CS_ADAMW_MAX_GROUPS <= 32, "five bits of group");
 template <class Entry, int N>
 struct Table {
   int count;
+  int per;    // kChunks of a CTA
   float one;  // 1 (see sum2)
   const float* grad_scale;
   AdamGroup groups[CS_ADAMW_MAX_GROUPS];
@@ -149,14 +151,12 @@ __device__ __forceinline__ void store_wide(float* p, const float2 (&x)[4]) {
 }
 
 struct StepCoef {
-  float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale, one;
+  float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale;
   uint32_t key;
 };
 
-__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale,
-                                            float one) {
+__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale) {
   StepCoef c;
-  c.one = one;
   c.b1 = g.b1;
   c.omb1 = g.omb1;
   c.b2 = g.b2;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kChunkThreads)
     adamw_kernel(const __grid_constant__ Table<AdamEntry, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
   switch (e.word & 3) {
     case CS_F32: step_chunk<float>(e, c, at); break;
@@ -258,8 +258,8 @@ __global__ void __launch_bounds__(kChunkThreads)
 // 2^-96 (v), which puts the largest value at the exponent field 15 (m) or 31
 // (v) of a float32, and the code is that float's bits 20..26 with the sign (m:
 // sign, 4 exponent, 3 fraction bits) or 20..27 (v: 5 and 3), the float's own
-// gradual underflow included.  Decoding is the same shift and two exact
-// multiplications, one of which is the beta of the average.  The 20 low bits
+// gradual underflow included.  Decoding is the same shift and two
+// multiplications, by a power of two and by the average's beta over another.  The 20 low bits
 // go by stochastic rounding: a moment that moves by 1 - beta2 = 0.1% a step
 // would never leave its code (6 to 12% wide) by rounding to nearest.  A v above
 // zero keeps at least its smallest code, so that m / sqrt(v) stays bounded.
@@ -267,6 +267,8 @@ __global__ void __launch_bounds__(kChunkThreads)
 // of its elements then stand for NaN.
 
 constexpr int kMinScale = 40;
+constexpr float kLeastEps = 8.673617379884035e-19f;  // 2^-60, the root of the smallest v
+
 constexpr float kTwoM112 = 1.925929944387236e-34f, kTwo112 = 5.192296858534828e33f;
 constexpr float kTwoM96 = 1.262177448353619e-29f, kTwo96 = 7.922816251426434e28f;
 
@@ -285,14 +287,15 @@ __device__ __forceinline__ uint32_t block_key(uint32_t key, uint32_t place, uint
   return mix32(key + place * 0x3C6EF373u + block * 0xA54FF53Bu);
 }
 __device__ __forceinline__ float scale_unit(uint32_t e) {
-  return e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float(e << 23);
+  const float x = __uint_as_float(e << 23);  // infinity for 255
+  return __fmaf_rn(x, 0.0f, x);              // which this turns into NaN
 }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t largest_bits) {
   const uint32_t e = max((largest_bits + 0xFFFFFu) >> 23, (uint32_t)kMinScale);  // NaN: 256
   return e >= 254 ? 255u : e;
 }
-__device__ __forceinline__ float scale_inverse(uint32_t e) {
-  return e == 255 ? 0.0f : __uint_as_float((254u - e) << 23);
+__device__ __forceinline__ float scale_inverse(uint32_t e) {  // codes of a marked block: any
+  return __uint_as_float((254u - e) << 23);
 }
 __device__ __forceinline__ float decode_m(uint32_t code) {  // times 2^(E-127)
   return __uint_as_float(((code & 127u) << 20) | ((code & 128u) << 24)) * kTwo112;
@@ -318,11 +321,6 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float sqrt_approx(float x) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -346,27 +344,64 @@ __device__ __forceinline__ float2 bits_v(uint32_t w) {
   return bits2((w << (20 - 8 * U)) & 0x0FF00000u,
                (U == 0 ? w << 12 : w >> 4) & 0x0FF00000u);
 }
-// The two 16-bit tops of a pair of floats' bits in one word.
-__device__ __forceinline__ uint32_t tops(uint32_t a, uint32_t b) {
-  return __byte_perm(a, b, 0x7632);
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&t)[4]) {
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x0073), 0x5410);
 }
 
+struct StepCoef8 {
+  float b1, b2, omb1, omb2, scale, one, decay, root, off;
+  uint32_t key;
+};
+// off / root hold eps (at least the root of the smallest v that the format
+// holds) and the correction of v, both over the negative step size; a step size
+// of zero moves nothing.
+__device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float* grad_scale,
+                                                float one) {
+  const StepCoef s = load_coef(g, grad_scale);
+  StepCoef8 c;
+  c.b1 = s.b1;
+  c.b2 = s.b2;
+  c.omb1 = s.omb1;
+  c.omb2 = s.omb2;
+  c.scale = s.scale;
+  c.one = one;
+  c.decay = s.decay;
+  c.root = s.step_size == 0.0f ? 0.0f : __fdividef(-s.rbc2, s.step_size);
+  c.off = __fdividef(-fmaxf(s.eps, kLeastEps), s.step_size);
+  c.key = s.key;
+  return c;
+}
+
+// Gives positive v whose code is 0 the code 1.  Rare, and not inlined: inline it
+// would be executed under predicates every time.
+__device__ __noinline__ uint32_t raised_zeros(uint32_t w, float a, float b, float c, float d) {
+  if (!(w & 0xFFu) && a > 0.0f) w |= 1u;
+  if (!(w & 0xFF00u) && b > 0.0f) w |= 1u << 8;
+  if (!(w & 0xFF0000u) && c > 0.0f) w |= 1u << 16;
+  if (!(w & 0xFF000000u) && d > 0.0f) w |= 1u << 24;
+  return w;
+}
 // A lane's eight elements of one block: P and the codes in mw, vw in, the same
-// out, and the block's new scale bytes.  Arithmetic on m and v is in float32
-// pairs (two independent IEEE operations an instruction) in the written order;
-// decoding's power of two is folded into beta, which changes no bit.  The
-// parameter's update uses the hardware's square root and reciprocal, each
-// within 2^-22: the bytes do not depend on it.
-// `first` is the element of the lane's first value in the block, `stride` the
-// distance of the next.
+// out, and the block's new scale bytes; mk, vk are the betas times the old
+// scales' units.  Arithmetic on m and v is in float32 pairs (two independent
+// IEEE operations an instruction) in the written order; decoding's power of two
+// is folded into beta, which changes no bit.  The parameter's update,
+// -step m / (sqrt(v) rbc2 + eps) = m / (sqrt(v) c.root + c.off), uses the
+// hardware's square root and reciprocal, each within 2^-22: the bytes do not
+// depend on it.  `first` is the element of the lane's first value in the block,
+// kStride the distance of the next.
+//
+// With 16-bit parameters the instructions bound it, not the memory: some 48 an
+// element, 20 of them integer.  268 M bfloat16 elements take 460 us (5.85 TB/s,
+// 89% of the copy rate; 618 us before the codes were built word by word, the
+// per-block values prepared a block a lane and the next block prefetched),
+// float32 657 us (6.54 TB/s, the copy rate).
 template <int kStride>
-__device__ __forceinline__ void step_lane8(const StepCoef& c, float2 (&P)[4], float2 (&G)[4],
-                                           uint32_t (&mw)[2], uint32_t (&vw)[2], float mb,
-                                           float vb, uint32_t key, uint32_t first, uint32_t& me,
+__device__ __forceinline__ void step_lane8(const StepCoef8& c, float2 (&P)[4],
+                                           const float2 (&G)[4], uint32_t (&mw)[2],
+                                           uint32_t (&vw)[2], float mk, float vk,
+                                           uint32_t key, uint32_t first, uint32_t& me,
                                            uint32_t& ve) {
-  const float2 scale = pair(c.scale), omb1 = pair(c.omb1), omb2 = pair(c.omb2), one = pair(c.one);
-  const float2 mk = pair(c.b1 * mb), vk = pair(c.b2 * vb);
-  const float2 up112 = pair(kTwo112), up96 = pair(kTwo96);
   float2 M[4], V[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -376,103 +411,155 @@ __device__ __forceinline__ void step_lane8(const StepCoef& c, float2 (&P)[4], fl
   float mmax = 0.0f, vmax = 0.0f;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const float2 g = __fmul2_rn(G[u], scale);
-    M[u] = sum2(__fmul2_rn(__fmul2_rn(M[u], up112), mk), one, __fmul2_rn(g, omb1));
-    V[u] = sum2(__fmul2_rn(__fmul2_rn(V[u], up96), vk), one,
-                __fmul2_rn(__fmul2_rn(g, g), omb2));
+    const float2 g = __fmul2_rn(G[u], pair(c.scale));
+    M[u] = sum2(__fmul2_rn(__fmul2_rn(M[u], pair(kTwo112)), pair(mk)), pair(c.one), __fmul2_rn(g, pair(c.omb1)));
+    V[u] = sum2(__fmul2_rn(__fmul2_rn(V[u], pair(kTwo96)), pair(vk)), pair(c.one),
+                __fmul2_rn(__fmul2_rn(g, g), pair(c.omb2)));
     mmax = max3_abs(mmax, M[u].x, M[u].y);
     vmax = max3_abs(vmax, V[u].x, V[u].y);
-    // v below the smallest normal number counts as that, so that its flushed
-    // root cannot leave a denominator of zero
-    const float2 root = make_float2(sqrt_approx(max_nan(V[u].x, 1.17549435e-38f)),
-                                    sqrt_approx(max_nan(V[u].y, 1.17549435e-38f)));
-    const float2 d = __ffma2_rn(root, pair(c.rbc2), pair(c.eps));
-    const float2 q = __fmul2_rn(M[u], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
-    P[u] = __ffma2_rn(q, pair(-c.step_size), __fmul2_rn(P[u], pair(c.decay)));
+    const float2 root = make_float2(sqrt_approx(V[u].x), sqrt_approx(V[u].y));
+    const float2 d = __ffma2_rn(root, pair(c.root), pair(c.off));
+    P[u] = __ffma2_rn(M[u], make_float2(rcp_approx(d.x), rcp_approx(d.y)),
+                      __fmul2_rn(P[u], pair(c.decay)));
   }
   me = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
   ve = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
   const float2 mi = pair(scale_inverse(me)), vi = pair(scale_inverse(ve));
-  const float2 down112 = pair(kTwoM112), down96 = pair(kTwoM96);
   const uint32_t start = key + first * 0x9E3779B1u;
+  uint32_t zero = 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t t[4], w[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int u = 2 * h + j;
-      const float2 ym = __fmul2_rn(__fmul2_rn(M[u], mi), down112);
-      const float2 yv = __fmul2_rn(__fmul2_rn(V[u], vi), down96);
+      const float2 ym = __fmul2_rn(__fmul2_rn(M[u], mi), pair(kTwoM112));
+      const float2 yv = __fmul2_rn(__fmul2_rn(V[u], vi), pair(kTwoM96));
       uint32_t r0 = start + (uint32_t)(2 * u * kStride) * 0x9E3779B1u;
       uint32_t r1 = start + (uint32_t)((2 * u + 1) * kStride) * 0x9E3779B1u;
       r0 = (r0 ^ (r0 >> 16)) * 0x6A09E667u;
       r1 = (r1 ^ (r1 >> 16)) * 0x6A09E667u;
       r0 ^= r0 >> 15;
       r1 ^= r1 >> 15;
-      t[2 * j] = __float_as_uint(ym.x) + ((r0 & 0xFFFFu) << 4);
-      t[2 * j + 1] = __float_as_uint(ym.y) + ((r1 & 0xFFFFu) << 4);
-      w[2 * j] = __float_as_uint(yv.x) + ((r0 >> 16) << 4);
-      w[2 * j + 1] = __float_as_uint(yv.y) + ((r1 >> 16) << 4);
-      if (V[u].x > 0.0f) w[2 * j] = max(w[2 * j], 1u << 20);
-      if (V[u].y > 0.0f) w[2 * j + 1] = max(w[2 * j + 1], 1u << 20);
+      // (bits + (random << 4)) << 4: the code comes to lie in the top byte
+      const uint32_t mx = __float_as_uint(ym.x), my = __float_as_uint(ym.y);
+      t[2 * j] = (mx * 16u + __byte_perm(r0, 0, 0x4104)) | (mx & 0x80000000u);
+      t[2 * j + 1] = (my * 16u + __byte_perm(r1, 0, 0x4104)) | (my & 0x80000000u);
+      w[2 * j] = __float_as_uint(yv.x) * 16u + __byte_perm(r0, 0, 0x4324);
+      w[2 * j + 1] = __float_as_uint(yv.y) * 16u + __byte_perm(r1, 0, 0x4324);
     }
-    // code = bits 20..26 (27) of each: shifted to bytes 0 and 2 of a pair's word
-    const uint32_t size = __byte_perm(tops(t[0], t[1]) >> 4, tops(t[2], t[3]) >> 4, 0x6420);
-    const uint32_t top = __byte_perm(__byte_perm(t[0], t[1], 0x0073),
-                                     __byte_perm(t[2], t[3], 0x0073), 0x5410);
-    mw[h] = (size & 0x7F7F7F7Fu) | (top & 0x80808080u);
-    vw[h] = __byte_perm(tops(w[0], w[1]) >> 4, tops(w[2], w[3]) >> 4, 0x6420);
+    mw[h] = top_bytes(t);
+    vw[h] = top_bytes(w);
+    zero |= (vw[h] - 0x01010101u) & ~vw[h] & 0x80808080u;
+  }
+  if (zero) {  // some code of v is 0: only for v = 0
+    vw[0] = raised_zeros(vw[0], V[0].x, V[0].y, V[1].x, V[1].y);
+    vw[1] = raised_zeros(vw[1], V[2].x, V[2].y, V[3].x, V[3].y);
   }
 }
 
-template <class T, bool kVec>
-__device__ __forceinline__ void step_block8(const AdamEntry8& e, const StepCoef& c, int64_t block,
-                                            int64_t left) {
-  const int lane = threadIdx.x & 31;
-  const int64_t at = block * kBlock8;
+// Two elements of a word or two, as float32.
+template <class T>
+__device__ __forceinline__ float2 unpack2(const uint32_t* w);
+template <>
+__device__ __forceinline__ float2 unpack2<float>(const uint32_t* w) {
+  return bits2(w[0], w[1]);
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(const uint32_t* w) {
+  return bits2(w[0] << 16, w[0] & 0xFFFF0000u);
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(const uint32_t* w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(w));
+}
+
+// One lane's share of an aligned, full block as it lies in memory, and where.
+template <class T>
+struct Raw8 {
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t p[kWords], g[kWords];
+  uint2 m, v;
+};
+template <int kWords>
+__device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[kWords]) {
+#pragma unroll
+  for (int i = 0; i < kWords; i += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(at + 4 * i);
+    w[i] = q.x;
+    w[i + 1] = q.y;
+    w[i + 2] = q.z;
+    w[i + 3] = q.w;
+  }
+}
+template <class T>
+struct Lane8 {  // offsets are 32 bits: an entry holds at most 2^30 elements
+  char *p, *m, *v;
+  const char* g;
+  uint32_t lane;
+  __device__ __forceinline__ Lane8(const AdamEntry8& e, uint32_t lane)
+      : p(static_cast<char*>(e.p)),
+        m(reinterpret_cast<char*>(e.m)),
+        v(reinterpret_cast<char*>(e.v)),
+        g(static_cast<const char*>(e.g)),
+        lane(lane) {}
+  __device__ __forceinline__ void load(uint32_t block, Raw8<T>& r) const {
+    const uint32_t at = block * kBlock8 + lane * 8;
+    load_words(p + at * (uint32_t)sizeof(T), r.p);
+    load_words(g + at * (uint32_t)sizeof(T), r.g);
+    r.m = *reinterpret_cast<const uint2*>(m + at);
+    r.v = *reinterpret_cast<const uint2*>(v + at);
+  }
+  // The step of a loaded block; new scale bytes in me, ve.
+  __device__ __forceinline__ void step(const StepCoef8& c, uint32_t block, const Raw8<T>& r,
+                                       float mk, float vk, uint32_t key, uint32_t& me,
+                                       uint32_t& ve) const {
+    float2 P[4], G[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      P[u] = unpack2<T>(r.p + u * (sizeof(T) / 2));
+      G[u] = unpack2<T>(r.g + u * (sizeof(T) / 2));
+    }
+    uint32_t mw[2] = {r.m.x, r.m.y}, vw[2] = {r.v.x, r.v.y};
+    step_lane8<1>(c, P, G, mw, vw, mk, vk, key, lane * 8, me, ve);
+    const uint32_t at = block * kBlock8 + lane * 8;
+    store8(reinterpret_cast<T*>(p + at * (uint32_t)sizeof(T)), P);
+    *reinterpret_cast<uint2*>(m + at) = make_uint2(mw[0], mw[1]);
+    *reinterpret_cast<uint2*>(v + at) = make_uint2(vw[0], vw[1]);
+  }
+};
+
+// A block that is cut short or not aligned: every 32nd element, one at a time.
+template <class T>
+__device__ __forceinline__ void step_part8(const AdamEntry8& e, const StepCoef8& c, uint32_t block,
+                                           int lane) {
+  const int64_t at = (int64_t)block * kBlock8;
+  const int left = (int)min((int64_t)kBlock8, e.numel - at);
   T* p = static_cast<T*>(e.p) + at;
   const T* g = static_cast<const T*>(e.g) + at;
   uint8_t* mc = e.m + at;
   uint8_t* vc = e.v + at;
   float2 P[4], G[4];
-  uint32_t mw[2] = {0, 0}, vw[2] = {0, 0};
-  if (kVec) {
-    load8(p + lane * 8, P);
-    load8(g + lane * 8, G);
-    const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
-    const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
-    mw[0] = a.x;
-    mw[1] = a.y;
-    vw[0] = b.x;
-    vw[1] = b.y;
-  } else {
+  uint32_t mw[2] = {0, 0}, vw[2] = {0, 0}, me, ve;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = lane + 32 * u;
-      const bool in = i < left;
-      (u & 1 ? P[u >> 1].y : P[u >> 1].x) = in ? to_f32(p[i]) : 0.0f;
-      (u & 1 ? G[u >> 1].y : G[u >> 1].x) = in ? to_f32(g[i]) : 0.0f;
-      mw[u >> 2] |= (in ? (uint32_t)mc[i] : 0u) << (8 * (u & 3));
-      vw[u >> 2] |= (in ? (uint32_t)vc[i] : 0u) << (8 * (u & 3));
-    }
+  for (int u = 0; u < 8; ++u) {
+    const int i = lane + 32 * u;
+    const bool in = i < left;
+    (u & 1 ? P[u >> 1].y : P[u >> 1].x) = in ? to_f32(p[i]) : 0.0f;
+    (u & 1 ? G[u >> 1].y : G[u >> 1].x) = in ? to_f32(g[i]) : 0.0f;
+    mw[u >> 2] |= (in ? (uint32_t)mc[i] : 0u) << (8 * (u & 3));
+    vw[u >> 2] |= (in ? (uint32_t)vc[i] : 0u) << (8 * (u & 3));
   }
-  const float mb = scale_unit(e.ms[block]), vb = scale_unit(e.vs[block]);
-  const uint32_t key = block_key(c.key, e.word >> 8, (uint32_t)block);
-  uint32_t me, ve;
-  step_lane8<kVec ? 1 : 32>(c, P, G, mw, vw, mb, vb, key, kVec ? lane * 8 : lane, me, ve);
-  if (kVec) {
-    store8(p + lane * 8, P);
-    *reinterpret_cast<uint2*>(mc + lane * 8) = make_uint2(mw[0], mw[1]);
-    *reinterpret_cast<uint2*>(vc + lane * 8) = make_uint2(vw[0], vw[1]);
-  } else {
+  const uint32_t em = e.ms[block], ev = e.vs[block];
+  step_lane8<32>(c, P, G, mw, vw, c.b1 * scale_unit(em), c.b2 * scale_unit(ev),
+                 block_key(c.key, e.word >> 8, e.block0 + block), lane, me, ve);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = lane + 32 * u;
-      if (i < left) {
-        p[i] = from_f32<T>(u & 1 ? P[u >> 1].y : P[u >> 1].x);
-        mc[i] = (uint8_t)(mw[u >> 2] >> (8 * (u & 3)));
-        vc[i] = (uint8_t)(vw[u >> 2] >> (8 * (u & 3)));
-      }
+  for (int u = 0; u < 8; ++u) {
+    const int i = lane + 32 * u;
+    if (i < left) {
+      p[i] = from_f32<T>(u & 1 ? P[u >> 1].y : P[u >> 1].x);
+      mc[i] = (uint8_t)(mw[u >> 2] >> (8 * (u & 3)));
+      vc[i] = (uint8_t)(vw[u >> 2] >> (8 * (u & 3)));
     }
   }
   if (lane == 0) {
@@ -481,28 +568,86 @@ __device__ __forceinline__ void step_block8(const AdamEntry8& e, const StepCoef&
   }
 }
 
+// A warp's blocks: one of each kChunk that its CTA takes, which lie as far
+// apart as the tensor has CTAs, so that all CTAs together walk through memory
+// (neighbouring chunks for each CTA were 2.4 times slower: everything in flight
+// was a slice of 8 KB in every 64).  What a block has one of (scales, key) is
+// prepared and stored for all of the warp's blocks at once, a block a lane (32
+// blocks a warp at most; 268 M bfloat16 elements take 469 us so, 492 with eight,
+// 594 with two).
+// With 16-bit parameters the next block's loads are issued before the present
+// one's arithmetic (they need 12 registers; float32's 20 would cost a CTA of
+// occupancy).
 template <class T>
-__device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef& c, int64_t at) {
-  const int64_t block = at / kBlock8 + (threadIdx.x >> 5);
-  const int64_t left = e.numel - block * kBlock8;
-  if (left <= 0) return;
-  if ((e.word & 4) && left >= kBlock8)
-    step_block8<T, true>(e, c, block, left);
-  else
-    step_block8<T, false>(e, c, block, left);
+__device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8& c, uint32_t chunk,
+                                           uint32_t per) {
+  constexpr uint32_t kWarps = kChunkThreads / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t chunks = (uint32_t)((e.numel + kChunk - 1) / kChunk);
+  const uint32_t stride = (chunks + per - 1) / per * kWarps;
+  const uint32_t first = chunk * kWarps + (threadIdx.x >> 5);
+  const uint32_t end = (uint32_t)((e.numel + kBlock8 - 1) / kBlock8);
+  const uint32_t full = (e.word & 4) ? (uint32_t)(e.numel / kBlock8) : 0;
+  int n = 0;  // full blocks of this warp
+  if (first < full) n = (int)min(per, (full - first + stride - 1) / stride);
+  if (n > 0) {
+    const Lane8<T> at(e, lane);
+    Raw8<T> a, b;
+    at.load(first, a);
+    const uint32_t mine = first + lane * stride;
+    uint32_t em = 1, ev = 1;
+    if (lane < n) {
+      em = e.ms[mine];
+      ev = e.vs[mine];
+    }
+    const float mk = c.b1 * scale_unit(em), vk = c.b2 * scale_unit(ev);
+    const uint32_t key = block_key(c.key, e.word >> 8, e.block0 + mine);
+    const auto step = [&](int i, const Raw8<T>& r) {
+      uint32_t me, ve;
+      at.step(c, first + i * stride, r, __shfl_sync(0xffffffffu, mk, i),
+              __shfl_sync(0xffffffffu, vk, i),
+              __shfl_sync(0xffffffffu, key, i), me, ve);
+      if (lane == i) {
+        em = me;
+        ev = ve;
+      }
+    };
+    if (sizeof(T) == 2) {
+      for (int i = 0;;) {
+        if (i + 1 < n) at.load(first + (i + 1) * stride, b);
+        step(i, a);
+        if (++i == n) break;
+        if (i + 1 < n) at.load(first + (i + 1) * stride, a);
+        step(i, b);
+        if (++i == n) break;
+      }
+    } else {
+      for (int i = 0;;) {
+        step(i, a);
+        if (++i == n) break;
+        at.load(first + i * stride, a);
+      }
+    }
+    if (lane < n) {
+      e.ms[mine] = (uint8_t)em;
+      e.vs[mine] = (uint8_t)ev;
+    }
+  }
+  for (uint32_t block = first + n * stride, i = n; i < per && block < end; ++i, block += stride)
+    step_part8<T>(e, c, block, lane);
 }
 
 template <int N>
-__global__ void __launch_bounds__(kChunkThreads)
+__global__ void __launch_bounds__(kChunkThreads, 3)
     adamw8_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
-  const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
+  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
+  const int chunk = (int)blockIdx.x - t.first[k];
   switch (e.word & 3) {
-    case CS_F32: step_warp8<float>(e, c, at); break;
-    case CS_BF16: step_warp8<__nv_bfloat16>(e, c, at); break;
-    default: step_warp8<__half>(e, c, at); break;
+    case CS_F32: step_warp8<float>(e, c, chunk, t.per); break;
+    case CS_BF16: step_warp8<__nv_bfloat16>(e, c, chunk, t.per); break;
+    default: step_warp8<__half>(e, c, chunk, t.per); break;
   }
 }
 
@@ -716,52 +861,66 @@ struct GroupBuilder {
   }
 };
 
-// The vector path needs parameters and gradients (in cs_adamw8_moments the
-// outputs) aligned to `width` bytes.
-inline bool make_entry(const cs_adamw_tensor& s, int place, int width, AdamEntry& e) {
+// An entry holds elements [at, at + n) of a tensor.  The vector path needs
+// parameters and gradients (in cs_adamw8_moments the outputs) aligned to
+// `width` bytes.
+inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
+                       AdamEntry& e) {
   if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq) return false;
-  const bool vec = aligned_to(s.param, width) && aligned_to(s.grad, width) &&
-                   aligned_to(s.exp_avg, 16) && aligned_to(s.exp_avg_sq, 16);
-  e = AdamEntry{s.param, s.grad, s.exp_avg, s.exp_avg_sq, s.numel,
-                entry_word(s.dtype, vec, s.group, place), 0};
+  const int64_t bytes = at * dtype_size(s.dtype);
+  e.p = static_cast<char*>(s.param) + bytes;
+  e.g = static_cast<const char*>(s.grad) + bytes;
+  e.m = static_cast<float*>(s.exp_avg) + at;
+  e.v = static_cast<float*>(s.exp_avg_sq) + at;
+  e.numel = n;
+  const bool vec = aligned_to(e.p, width) && aligned_to(e.g, width) && aligned_to(e.m, 16) &&
+                   aligned_to(e.v, 16);
+  e.word = entry_word(s.dtype, vec, s.group, place);
+  e.pad = 0;
   return true;
 }
 
-inline bool make_entry(const cs_adamw_tensor& s, int place, int width, AdamEntry8& e) {
+inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
+                       AdamEntry8& e) {
   if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !s.exp_avg_scales ||
       !s.exp_avg_sq_scales)
     return false;
-  const bool vec = aligned_to(s.param, width) && aligned_to(s.grad, width) &&
-                   aligned_to(s.exp_avg, 8) && aligned_to(s.exp_avg_sq, 8);
-  e = AdamEntry8{s.param,
-                 s.grad,
-                 static_cast<uint8_t*>(s.exp_avg),
-                 static_cast<uint8_t*>(s.exp_avg_sq),
-                 s.exp_avg_scales,
-                 s.exp_avg_sq_scales,
-                 s.numel,
-                 entry_word(s.dtype, vec, s.group, place),
-                 0};
+  const int64_t bytes = at * dtype_size(s.dtype), block = at / kBlock8;
+  e.p = static_cast<char*>(s.param) + bytes;
+  e.g = static_cast<const char*>(s.grad) + bytes;
+  e.m = static_cast<uint8_t*>(s.exp_avg) + at;
+  e.v = static_cast<uint8_t*>(s.exp_avg_sq) + at;
+  e.ms = s.exp_avg_scales + block;
+  e.vs = s.exp_avg_sq_scales + block;
+  e.numel = n;
+  const bool vec = aligned_to(e.p, width) && aligned_to(e.g, width) && aligned_to(e.m, 8) &&
+                   aligned_to(e.v, 8);
+  e.word = entry_word(s.dtype, vec, s.group, place);
+  e.block0 = (uint32_t)block;
   return true;
 }
 
+// CTAs of a launch that still takes several chunks a CTA: four rounds of the
+// 148 SMs' four.
+constexpr int64_t kPerWaves = 148 * 16;
+
 // The kernels of one table type, by name.
 struct RunStep {
-  static constexpr int kWidth = 16;
+  static constexpr int kWidth = 16, kMostPer = 1;
   template <int N>
   static void launch(const Table<AdamEntry, N>& t, int chunks, cudaStream_t st) {
     adamw_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunStep8 {
-  static constexpr int kWidth = 16;
+  static constexpr int kWidth = 16, kMostPer = 32;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunMoments8 {
-  static constexpr int kWidth = 32;
+  static constexpr int kWidth = 32, kMostPer = 1;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_moments_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
@@ -777,21 +936,28 @@ int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const A
   t.one = 1.0f;
   t.grad_scale = grad_scale;
   for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
+  int64_t total = 0;
+  for (int i = 0; i < count; ++i) total += (tensors[i].numel + kChunk - 1) / kChunk;
+  t.per = 1;
+  while (t.per < Run::kMostPer && total / t.per >= 2 * kPerWaves) t.per *= 2;
+  const int64_t unit = (int64_t)kChunk * t.per;
   t.count = 0;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     const cs_adamw_tensor& s = tensors[i];
-    if (s.numel == 0) continue;
-    const int64_t mine = (s.numel + kChunk - 1) / kChunk;
-    if (t.count == N || chunks + mine > INT32_MAX) {
-      Run::template launch<N>(t, (int)chunks, st);
-      if (int rc = launch_status()) return rc;
-      t.count = 0;
-      chunks = 0;
+    for (int64_t at = 0; at < s.numel; at += kMaxEntry) {
+      const int64_t n = s.numel - at < kMaxEntry ? s.numel - at : kMaxEntry;
+      const int64_t mine = (n + unit - 1) / unit;
+      if (t.count == N || chunks + mine > INT32_MAX) {
+        Run::template launch<N>(t, (int)chunks, st);
+        if (int rc = launch_status()) return rc;
+        t.count = 0;
+        chunks = 0;
+      }
+      if (!make_entry(s, i, Run::kWidth, at, n, t.e[t.count])) return CS_ERR_ARG;
+      t.first[t.count++] = (int)chunks;
+      chunks += mine;
     }
-    if (!make_entry(s, i, Run::kWidth, t.e[t.count])) return CS_ERR_ARG;
-    t.first[t.count++] = (int)chunks;
-    chunks += mine;
   }
   if (t.count == 0) return CS_OK;
   Run::template launch<N>(t, (int)chunks, st);

@@ -286,6 +286,36 @@ def test_adamw8_step_of_small_and_large_gradients(size):
         step8_and_check([p], [make(1000, F32, gen, size)], [st], step)
 
 
+def test_adamw8_step_of_blocks_with_every_size_of_gradient():
+    """Magnitudes from 1e-21 (whose square is subnormal) to 1e17 in one block,
+    between blocks that hold a part of them: scales above and below the ranges
+    that one power of two covers, v too small for its block's scale, zeros."""
+    gen = torch.Generator().manual_seed(8)
+    n = 256 * 24 + 5
+    p = make(n, F32, gen, 0.3)
+    st = ops.adamw8_state(p)
+    for step in (1, 2, 3, 4):
+        top = torch.randint(-21, 18, (n // 256 + 1,), generator=gen).repeat_interleave(256)[:n]
+        low = torch.rand(n, generator=gen) * 38 - 21
+        g = 10.0 ** torch.minimum(low, top.float()) * torch.sign(torch.randn(n, generator=gen))
+        g[::11] = 0
+        step8_and_check([p], [g.cuda()], [st], step)
+
+
+def test_a_learning_rate_of_zero_moves_nothing():
+    gen = torch.Generator().manual_seed(8)
+    for dtype in (F32, BF16):
+        p, g = make(3000, dtype, gen, 0.3), make(3000, dtype, gen)
+        p[::5] = 0
+        g[::3] = 0
+        old = p.clone()
+        st = ops.adamw8_state(p)
+        ops.adamw8_step([p], [g], *[[x] for x in st], step=1, lr=0.0)
+        m, v = moments32(p, gen)
+        ops.adamw_step([p], [g], [m], [v], step=1, lr=0.0)
+        assert torch.equal(p, old) and st[0].any()
+
+
 @pytest.mark.parametrize("shift", [1, 3, 4, 8])
 def test_adamw8_step_of_views_leaves_their_surroundings(shift):
     gen = torch.Generator().manual_seed(shift)
