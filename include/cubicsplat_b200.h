@@ -449,9 +449,10 @@ typedef struct cs_grad_tensor {
 
 /* norm = sqrt of the sum of squares over all tensors, accumulated in double;
  * scale (may be NULL) = min(1, max_norm / (norm + eps)), or 1 for max_norm <= 0.
- * Workspace: cs_grad_norm_workspace_size(count) bytes, 8-byte aligned, in any
- * state, not shared with a call that may run at the same time. */
-CS_API size_t cs_grad_norm_workspace_size(int32_t count);
+ * Workspace: cs_grad_norm_workspace_size bytes (0 for few elements, which take
+ * one launch; it may be NULL then), 8-byte aligned, in any state, not shared with
+ * a call that may run at the same time. */
+CS_API size_t cs_grad_norm_workspace_size(const cs_grad_tensor *tensors, int32_t count);
 CS_API int cs_grad_norm(const cs_grad_tensor *tensors, int32_t count, double max_norm, double eps,
                  float *norm, float *scale, void *workspace, void *stream);
 

@@ -87,7 +87,7 @@ SIGNATURES = {
     "cs_adamw8_step": (ctypes.c_int, [_P, _I32, _P, _I32, _P, ctypes.c_uint32, _P, _P]),
     "cs_adamw8_moments": (ctypes.c_int, [_P, _I32, _P]),
     "cs_adamw_advance": (ctypes.c_int, [_P, _P, _I32, ctypes.c_uint32, _P, _P]),
-    "cs_grad_norm_workspace_size": (_SZ, [_I32]),
+    "cs_grad_norm_workspace_size": (_SZ, [_P, _I32]),
     "cs_grad_norm": (ctypes.c_int, [_P, _I32, ctypes.c_double, ctypes.c_double, _P, _P, _P, _P]),
     "cs_ring_segments_forward": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),
     "cs_ring_segments_backward": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I32, _I32, _P]),

@@ -6,9 +6,15 @@
  * here, on the host, before anything is launched.  A call of any number of
  * tensors is one binding call.  Work runs on the current torch stream of the
  * tensors' device; temporaries come from torch's caching allocator.
+ *
+ * With hundreds of small tensors this reading is what bounds a call (1800
+ * tensors in an 8-bit step of 300 parameters), so it is one pass over all lists
+ * that works on the tensor implementations, and a tensor with the dispatch keys,
+ * type and device of the one before it is taken without further questions.
  */
 #include <torch/extension.h>
 
+#include <c10/core/impl/COW.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -35,11 +41,16 @@ void check(int status, const char* what) {
     throw std::runtime_error(std::string(what) + " failed (status " + std::to_string(status) + ")");
 }
 
+using Impl = c10::TensorImpl;
+
 // A sequence of tensors, read without copies while `seq` lives.
 struct TensorList {
   PyObject* fast;
+  PyObject** items;
   Py_ssize_t n;
   const char* name;
+  c10::DispatchKeySet keys;  // of the last tensor that passed all questions
+  caffe2::TypeMeta type;
   TensorList(const py::handle& seq, const char* what) : name(what) {
     fast = THPVariable_Check(seq.ptr()) ? nullptr : PySequence_Fast(seq.ptr(), "");
     if (!fast) {
@@ -47,17 +58,41 @@ struct TensorList {
       bad(std::string(what) + " must be a sequence of tensors");
     }
     n = PySequence_Fast_GET_SIZE(fast);
+    items = PySequence_Fast_ITEMS(fast);
   }
   TensorList(const TensorList&) = delete;
   TensorList& operator=(const TensorList&) = delete;
   ~TensorList() { Py_XDECREF(fast); }
   std::string at(Py_ssize_t i) const { return std::string(name) + "[" + std::to_string(i) + "]"; }
   const Tensor& operator[](Py_ssize_t i) const {
-    PyObject* o = PySequence_Fast_GET_ITEM(fast, i);
-    if (!THPVariable_Check(o)) bad(at(i) + " must be a tensor");
-    return THPVariable_Unpack(o);
+    if (!THPVariable_Check(items[i])) bad(at(i) + " must be a tensor");
+    return THPVariable_Unpack(items[i]);
+  }
+  // The tensor's implementation: dense, on `dev`, of one of the types that
+  // `takes` accepts (it names them otherwise).
+  template <class Takes>
+  Impl* get(Py_ssize_t i, const at::Device& dev, const Takes& takes) {
+    Impl* x = (*this)[i].unsafeGetTensorImpl();
+    if (x->key_set() == keys && x->dtype() == type && x->device() == dev) return x;
+    if (x->layout() != at::kStrided) bad(at(i) + " must be a dense tensor");
+    if (!x->is_cuda()) bad(at(i) + " must be a CUDA tensor");
+    if (x->device() != dev)
+      bad(at(i) + " must be on " + dev.str() + ", got " + x->device().str());
+    if (const char* want = takes(x->dtype().toScalarType()))
+      bad(at(i) + " must be " + want + ", got " + c10::toString(x->dtype().toScalarType()));
+    keys = x->key_set();
+    type = x->dtype();
+    return x;
   }
 };
+
+const char* takes_float(at::ScalarType t) {
+  return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf
+             ? nullptr
+             : "float32, bfloat16 or float16";
+}
+const char* takes_float32(at::ScalarType t) { return t == at::kFloat ? nullptr : "Float"; }
+const char* takes_byte(at::ScalarType t) { return t == at::kByte ? nullptr : "Byte"; }
 
 void same_length(const TensorList& a, const TensorList& b) {
   if (a.n != b.n)
@@ -65,43 +100,53 @@ void same_length(const TensorList& a, const TensorList& b) {
         std::to_string(a.n) + "), got " + std::to_string(b.n));
 }
 
-int dtype_code(const Tensor& t, const TensorList& l, Py_ssize_t i) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return CS_F32;
-    case at::kBFloat16: return CS_BF16;
-    case at::kHalf: return CS_F16;
-    default: bad(l.at(i) + " must be float32, bfloat16 or float16");
-  }
+int dtype_code(const Impl* x) {
+  const at::ScalarType t = x->dtype().toScalarType();
+  return t == at::kFloat ? CS_F32 : t == at::kBFloat16 ? CS_BF16 : CS_F16;
 }
 
-void on_device(const Tensor& t, const at::Device& dev, const TensorList& l, Py_ssize_t i) {
-  if (t.layout() != at::kStrided) bad(l.at(i) + " must be a dense tensor");
-  if (!t.is_cuda()) bad(l.at(i) + " must be a CUDA tensor");
-  if (t.device() != dev) bad(l.at(i) + " must be on " + dev.str() + ", got " + t.device().str());
+// The device of a list's first tensor, which has to be a CUDA tensor.
+at::Device device_of(TensorList& l) {
+  const Tensor& t = l[0];
+  if (t.layout() != at::kStrided) bad(l.at(0) + " must be a dense tensor");
+  if (!t.is_cuda()) bad(l.at(0) + " must be a CUDA tensor");
+  return t.device();
 }
 
-// Both tensors keep the same element at the same place of their storage.
-bool same_layout(const Tensor& a, const Tensor& b) {
-  return a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous());
+bool same_shape(const Impl* a, const Impl* b) {
+  const auto x = a->sizes(), y = b->sizes();
+  if (x.size() != y.size()) return false;
+  for (size_t i = 0; i < x.size(); ++i)
+    if (x[i] != y[i]) return false;
+  return true;
 }
 
-void like_param(const Tensor& t, const Tensor& p, at::ScalarType type, const TensorList& l,
+// Both tensors keep the same element at the same place of their storage;
+// `contiguous` says whether b is contiguous.
+bool same_layout(const Impl* a, const Impl* b, bool contiguous) {
+  return (contiguous && a->is_contiguous()) || a->strides() == b->strides();
+}
+
+// The tensor's memory (an elements-less tensor has none): the storage's pointer
+// itself, unless it is still shared copy-on-write and has to be made its own.
+void* data_of(Impl* x) {
+  if (!x->has_storage()) return x->mutable_data();  // which says why there is none
+  const at::DataPtr& p = x->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks();
+  if (!p.get() || c10::impl::cow::is_cow_data_ptr(p)) return x->mutable_data();
+  return static_cast<char*>(p.get()) + x->storage_offset() * x->itemsize();
+}
+
+void check_like(const Impl* x, const Impl* p, bool contiguous, const TensorList& l,
                 Py_ssize_t i) {
-  on_device(t, p.device(), l, i);
-  if (t.scalar_type() != type)
-    bad(l.at(i) + " must be " + std::string(c10::toString(type)) + ", got " +
-        c10::toString(t.scalar_type()));
-  if (t.sizes() != p.sizes() || !same_layout(t, p))
+  if (!same_shape(x, p) || !same_layout(x, p, contiguous))
     bad(l.at(i) + " must have its parameter's shape and strides");
 }
 
 int64_t scale_count(int64_t numel) { return (numel + CS_ADAMW8_BLOCK - 1) / CS_ADAMW8_BLOCK; }
 
-void check_scales(const Tensor& t, int64_t numel, const at::Device& dev, const TensorList& l,
-                  Py_ssize_t i) {
-  on_device(t, dev, l, i);
-  if (t.scalar_type() != at::kByte || !t.is_contiguous() || t.numel() != scale_count(numel))
-    bad(l.at(i) + " must be " + std::to_string(scale_count(numel)) +
+void check_scales(const Impl* x, int64_t count, const TensorList& l, Py_ssize_t i) {
+  if (!x->is_contiguous() || x->numel() != count)
+    bad(l.at(i) + " must be " + std::to_string(count) +
         " contiguous uint8 scales (one per started block of " + std::to_string(CS_ADAMW8_BLOCK) +
         " elements)");
 }
@@ -209,35 +254,33 @@ std::optional<Tensor> advance(const Groups& r, uint32_t seed, const at::Device& 
   return coef;
 }
 
-void written_param(const Tensor& p) {
-  if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+void written_impl(Impl* x) {
+  if (!x->is_inference()) x->bump_version();
 }
 
-// Parameters and gradients of a call; a gradient of another layout is copied.
-void read_params(const TensorList& params, const TensorList& grads,
-                 std::vector<cs_adamw_tensor>& out, std::vector<Tensor>& copies,
-                 const at::Device& dev, Written& written) {
-  for (Py_ssize_t i = 0; i < params.n; ++i) {
-    const Tensor& p = params[i];
-    const Tensor& g = grads[i];
-    on_device(p, dev, params, i);
-    cs_adamw_tensor& s = out[i];
-    s.dtype = dtype_code(p, params, i);
-    if (!p.is_non_overlapping_and_dense())
-      bad(params.at(i) + " must be non-overlapping and dense");
-    on_device(g, dev, grads, i);
-    if (g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes())
-      bad(grads.at(i) + " must have its parameter's shape and type");
-    s.numel = p.numel();
-    s.param = s.numel ? p.data_ptr() : nullptr;
-    if (same_layout(g, p) && !g.is_neg()) {
-      s.grad = s.numel ? g.data_ptr() : nullptr;
-    } else {
-      copies.push_back(at::empty_like(p).copy_(g));
-      s.grad = s.numel ? copies.back().data_ptr() : nullptr;
-    }
-    written.add(s.param, params, i);
+// A parameter and its gradient; a gradient of another layout is copied.
+// Returns whether the parameter is contiguous.
+bool read_param(TensorList& params, TensorList& grads, Py_ssize_t i, const at::Device& dev,
+                cs_adamw_tensor& s, Impl*& p, std::vector<Tensor>& copies, Written& written) {
+  p = params.get(i, dev, takes_float);
+  const bool contiguous = p->is_contiguous();
+  if (!contiguous && !p->is_non_overlapping_and_dense())
+    bad(params.at(i) + " must be non-overlapping and dense");
+  Impl* g = grads.get(i, dev, takes_float);
+  if (g->dtype() != p->dtype() || !same_shape(g, p))
+    bad(grads.at(i) + " must have its parameter's shape and type");
+  s.dtype = dtype_code(p);
+  s.numel = p->numel();
+  if (!s.numel) return contiguous;
+  s.param = data_of(p);
+  if (same_layout(g, p, contiguous) && !g->is_neg()) {
+    s.grad = data_of(g);
+  } else {
+    copies.push_back(at::empty_like(params[i]).copy_(grads[i]));
+    s.grad = copies.back().data_ptr();
   }
+  written.add(s.param, params, i);
+  return contiguous;
 }
 
 void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
@@ -251,30 +294,29 @@ void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
 void adamw_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
                 const py::object& exp_avg_sqs_, const py::list& groups,
                 const std::optional<Tensor>& grad_scale) {
-  const TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
+  TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       v(exp_avg_sqs_, "exp_avg_sqs");
-  same_length(params, grads);
-  same_length(params, m);
-  same_length(params, v);
+  for (const TensorList* l : {&grads, &m, &v}) same_length(params, *l);
   if (params.n == 0) return;
-  const at::Device dev = params[0].device();
-  const Groups r = read_groups(groups, params.n, dev);
-  on_device(params[0], dev, params, 0);
+  const Groups r = read_groups(groups, params.n, params[0].device());
+  const at::Device dev = device_of(params);
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
+  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
   Written written(3 * params.n);
-  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
-  read_params(params, grads, t, copies, dev, written);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
-    like_param(m[i], params[i], at::kFloat, m, i);
-    like_param(v[i], params[i], at::kFloat, v, i);
-    if (!t[i].numel) continue;
-    t[i].exp_avg = m[i].data_ptr();
-    t[i].exp_avg_sq = v[i].data_ptr();
-    written.add(t[i].exp_avg, m, i);
-    written.add(t[i].exp_avg_sq, v, i);
+    cs_adamw_tensor& s = t[i];
+    Impl* p;
+    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, written);
+    Impl* mi = m.get(i, dev, takes_float32);
+    Impl* vi = v.get(i, dev, takes_float32);
+    check_like(mi, p, contiguous, m, i);
+    check_like(vi, p, contiguous, v, i);
+    if (!s.numel) continue;
+    written.add(s.exp_avg = data_of(mi), m, i);
+    written.add(s.exp_avg_sq = data_of(vi), v, i);
   }
   set_groups(r, t);
   const std::optional<Tensor> coef = advance(r, 0, dev);
@@ -282,42 +324,43 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
                       coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
                       stream_of(dev)),
         "cs_adamw_step");
-  for (Py_ssize_t i = 0; i < params.n; ++i) written_param(params[i]);
+  for (Py_ssize_t i = 0; i < params.n; ++i) written_impl(params[i].unsafeGetTensorImpl());
 }
 
 void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
                  const py::object& m_scales_, const py::object& exp_avg_sqs_,
                  const py::object& v_scales_, const py::list& groups, uint32_t seed,
                  const std::optional<Tensor>& grad_scale) {
-  const TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
+  TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       ms(m_scales_, "exp_avg_scales"), v(exp_avg_sqs_, "exp_avg_sqs"),
       vs(v_scales_, "exp_avg_sq_scales");
   for (const TensorList* l : {&grads, &m, &ms, &v, &vs}) same_length(params, *l);
   if (params.n == 0) return;
-  const at::Device dev = params[0].device();
-  const Groups r = read_groups(groups, params.n, dev);
-  on_device(params[0], dev, params, 0);
+  const Groups r = read_groups(groups, params.n, params[0].device());
+  const at::Device dev = device_of(params);
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
+  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
   Written written(5 * params.n);
-  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
-  read_params(params, grads, t, copies, dev, written);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
-    like_param(m[i], params[i], at::kByte, m, i);
-    like_param(v[i], params[i], at::kByte, v, i);
-    check_scales(ms[i], t[i].numel, dev, ms, i);
-    check_scales(vs[i], t[i].numel, dev, vs, i);
-    if (!t[i].numel) continue;
-    t[i].exp_avg = m[i].data_ptr();
-    t[i].exp_avg_sq = v[i].data_ptr();
-    t[i].exp_avg_scales = static_cast<uint8_t*>(ms[i].data_ptr());
-    t[i].exp_avg_sq_scales = static_cast<uint8_t*>(vs[i].data_ptr());
-    written.add(t[i].exp_avg, m, i);
-    written.add(t[i].exp_avg_sq, v, i);
-    written.add(t[i].exp_avg_scales, ms, i);
-    written.add(t[i].exp_avg_sq_scales, vs, i);
+    cs_adamw_tensor& s = t[i];
+    Impl* p;
+    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, written);
+    Impl* mi = m.get(i, dev, takes_byte);
+    Impl* vi = v.get(i, dev, takes_byte);
+    check_like(mi, p, contiguous, m, i);
+    check_like(vi, p, contiguous, v, i);
+    Impl* msi = ms.get(i, dev, takes_byte);
+    Impl* vsi = vs.get(i, dev, takes_byte);
+    check_scales(msi, scale_count(s.numel), ms, i);
+    check_scales(vsi, scale_count(s.numel), vs, i);
+    if (!s.numel) continue;
+    written.add(s.exp_avg = data_of(mi), m, i);
+    written.add(s.exp_avg_sq = data_of(vi), v, i);
+    written.add(s.exp_avg_scales = static_cast<uint8_t*>(data_of(msi)), ms, i);
+    written.add(s.exp_avg_sq_scales = static_cast<uint8_t*>(data_of(vsi)), vs, i);
   }
   set_groups(r, t);
   const std::optional<Tensor> coef = advance(r, seed, dev);
@@ -325,82 +368,84 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
                        coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed, scale,
                        stream_of(dev)),
         "cs_adamw8_step");
-  for (Py_ssize_t i = 0; i < params.n; ++i) written_param(params[i]);
+  for (Py_ssize_t i = 0; i < params.n; ++i) written_impl(params[i].unsafeGetTensorImpl());
 }
 
 void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
                     const py::object& exp_avg_sqs_, const py::object& v_scales_,
                     const py::object& out_m_, const py::object& out_v_) {
-  const TensorList m(exp_avgs_, "exp_avgs"), ms(m_scales_, "exp_avg_scales"),
+  TensorList m(exp_avgs_, "exp_avgs"), ms(m_scales_, "exp_avg_scales"),
       v(exp_avg_sqs_, "exp_avg_sqs"), vs(v_scales_, "exp_avg_sq_scales"), om(out_m_, "out[0]"),
       ov(out_v_, "out[1]");
   for (const TensorList* l : {&ms, &v, &vs, &om, &ov}) same_length(m, *l);
   if (m.n == 0) return;
-  const at::Device dev = m[0].device();
-  on_device(m[0], dev, m, 0);
+  const at::Device dev = device_of(m);
   c10::cuda::CUDAGuard guard(dev);
   std::vector<cs_adamw_tensor> t(m.n, cs_adamw_tensor{});
   Written written(2 * m.n);
   for (Py_ssize_t i = 0; i < m.n; ++i) {
-    const Tensor& c = m[i];
-    on_device(c, dev, m, i);
-    if (c.scalar_type() != at::kByte || !c.is_non_overlapping_and_dense())
-      bad(m.at(i) + " must be non-overlapping, dense uint8 codes");
-    like_param(v[i], c, at::kByte, v, i);
-    like_param(om[i], c, at::kFloat, om, i);
-    like_param(ov[i], c, at::kFloat, ov, i);
-    check_scales(ms[i], c.numel(), dev, ms, i);
-    check_scales(vs[i], c.numel(), dev, vs, i);
-    t[i].numel = c.numel();
-    t[i].dtype = CS_F32;
-    if (!t[i].numel) continue;
-    t[i].param = om[i].data_ptr();
-    t[i].grad = ov[i].data_ptr();
-    t[i].exp_avg = c.data_ptr();
-    t[i].exp_avg_sq = v[i].data_ptr();
-    t[i].exp_avg_scales = static_cast<uint8_t*>(ms[i].data_ptr());
-    t[i].exp_avg_sq_scales = static_cast<uint8_t*>(vs[i].data_ptr());
-    written.add(t[i].param, om, i);
-    written.add(t[i].grad, ov, i);
+    cs_adamw_tensor& s = t[i];
+    Impl* c = m.get(i, dev, takes_byte);
+    const bool contiguous = c->is_contiguous();
+    if (!contiguous && !c->is_non_overlapping_and_dense())
+      bad(m.at(i) + " must be non-overlapping and dense");
+    Impl* vi = v.get(i, dev, takes_byte);
+    Impl* omi = om.get(i, dev, takes_float32);
+    Impl* ovi = ov.get(i, dev, takes_float32);
+    check_like(vi, c, contiguous, v, i);
+    check_like(omi, c, contiguous, om, i);
+    check_like(ovi, c, contiguous, ov, i);
+    Impl* msi = ms.get(i, dev, takes_byte);
+    Impl* vsi = vs.get(i, dev, takes_byte);
+    s.numel = c->numel();
+    s.dtype = CS_F32;
+    check_scales(msi, scale_count(s.numel), ms, i);
+    check_scales(vsi, scale_count(s.numel), vs, i);
+    if (!s.numel) continue;
+    s.exp_avg = data_of(c);
+    s.exp_avg_sq = data_of(vi);
+    s.exp_avg_scales = static_cast<uint8_t*>(data_of(msi));
+    s.exp_avg_sq_scales = static_cast<uint8_t*>(data_of(vsi));
+    written.add(s.param = data_of(omi), om, i);
+    written.add(s.grad = data_of(ovi), ov, i);
   }
   check(cs_adamw8_moments(t.data(), (int32_t)t.size(), stream_of(dev)), "cs_adamw8_moments");
   for (Py_ssize_t i = 0; i < m.n; ++i) {
-    written_param(om[i]);
-    written_param(ov[i]);
+    written_impl(om[i].unsafeGetTensorImpl());
+    written_impl(ov[i].unsafeGetTensorImpl());
   }
 }
 
 std::tuple<Tensor, Tensor> grad_norm(const py::object& grads_, double max_norm, double eps) {
-  const TensorList grads(grads_, "grads");
+  TensorList grads(grads_, "grads");
   if (grads.n == 0) bad("grads must not be empty");
   if (!(max_norm >= 0.0)) bad("Invalid max_norm: " + std::to_string(max_norm));
   if (!(eps >= 0.0)) bad("Invalid epsilon value: " + std::to_string(eps));
-  const at::Device dev = grads[0].device();
-  on_device(grads[0], dev, grads, 0);
+  const at::Device dev = device_of(grads);
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
   std::vector<cs_grad_tensor> t(grads.n, cs_grad_tensor{});
   std::vector<Tensor> copies;
   for (Py_ssize_t i = 0; i < grads.n; ++i) {
-    const Tensor& g = grads[i];
-    on_device(g, dev, grads, i);
-    t[i].dtype = dtype_code(g, grads, i);
-    t[i].numel = g.numel();
+    Impl* g = grads.get(i, dev, takes_float);
+    t[i].dtype = dtype_code(g);
+    t[i].numel = g->numel();
     if (!t[i].numel) continue;
-    if (g.is_non_overlapping_and_dense()) {
-      t[i].data = g.data_ptr();
+    if (g->is_contiguous() || g->is_non_overlapping_and_dense()) {
+      t[i].data = data_of(g);
     } else {
-      copies.push_back(g.contiguous());
+      copies.push_back(grads[i].contiguous());
       t[i].data = copies.back().data_ptr();
     }
   }
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
   Tensor norm = at::empty({}, f32), scale = at::empty({}, f32);
-  Tensor ws = at::empty({(int64_t)cs_grad_norm_workspace_size((int32_t)grads.n)},
-                        f32.dtype(at::kByte));
+  const size_t bytes = cs_grad_norm_workspace_size(t.data(), (int32_t)t.size());
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
   check(cs_grad_norm(t.data(), (int32_t)t.size(), max_norm, eps,
                      static_cast<float*>(norm.data_ptr()), static_cast<float*>(scale.data_ptr()),
-                     ws.data_ptr(), stream_of(dev)),
+                     bytes ? ws.data_ptr() : nullptr, stream_of(dev)),
         "cs_grad_norm");
   return {norm, scale};
 }

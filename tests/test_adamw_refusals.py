@@ -83,8 +83,10 @@ def test_c_entries_refuse_missing_scales_counters_and_workspaces():
                            (same, 17, 64)):
         assert nat.call("cs_adamw_advance", ctypes.addressof(steps), ctypes.addressof(g), n, 0,
                         coef, None) == CS_ERR_ARG
-    n = (CGrad * 1)(CGrad(256, 4, 0, 0))
+    n = (CGrad * 1)(CGrad(256, 1 << 30, 0, 0))  # large enough to need a workspace
     at = ctypes.addressof(n)
+    assert nat.call("cs_grad_norm_workspace_size", at, 1) >= 8
+    assert nat.call("cs_grad_norm_workspace_size", at, 0) == 0
     for args in ((at, -1, 64, 64, 64), (None, 1, 64, 64, 64), (at, 1, None, 64, 64),
                  (at, 1, 64, 64, None), (at, 1, 64, 64, 68)):
         assert nat.call("cs_grad_norm", args[0], args[1], 1.0, 1e-6, *args[2:], None) == CS_ERR_ARG
@@ -92,8 +94,8 @@ def test_c_entries_refuse_missing_scales_counters_and_workspaces():
         n = (CGrad * 1)(bad)
         assert nat.call("cs_grad_norm", ctypes.addressof(n), 1, 1.0, 1e-6, 64, 64, 64,
                         None) == CS_ERR_ARG
-    assert nat.call("cs_grad_norm_workspace_size", 0) >= 8
-    assert nat.call("cs_grad_norm_workspace_size", 1000) >= 8
+    few = (CGrad * 1)(CGrad(256, 1000, 0, 0))
+    assert nat.call("cs_grad_norm_workspace_size", ctypes.addressof(few), 1) == 0
 
 
 def _lists(k=2):
