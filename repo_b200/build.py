@@ -111,7 +111,7 @@ def build_torch_ext(force: bool = False) -> str:
     if not force and not _stale(EXT_PATH, deps):
         return EXT_PATH
     torch_lib = ce.library_paths()[0]
-    flags = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+    flags = [os.environ.get("CXX", "g++"), "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
              "-DTORCH_EXTENSION_NAME=_cs_torch", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     for inc in ce.include_paths() + [sysconfig.get_paths()["include"],

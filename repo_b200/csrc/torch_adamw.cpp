@@ -51,6 +51,7 @@ struct TensorList {
   const char* name;
   c10::DispatchKeySet keys;  // of the last tensor that passed all questions
   caffe2::TypeMeta type;
+  int64_t bytes = 0;  // of an element
   TensorList(const py::handle& seq, const char* what) : name(what) {
     fast = THPVariable_Check(seq.ptr()) ? nullptr : PySequence_Fast(seq.ptr(), "");
     if (!fast) {
@@ -82,7 +83,20 @@ struct TensorList {
       bad(at(i) + " must be " + want + ", got " + c10::toString(x->dtype().toScalarType()));
     keys = x->key_set();
     type = x->dtype();
+    bytes = (int64_t)type.itemsize();
     return x;
+  }
+  // The memory of a tensor that get() returned: its storage's, unless that is
+  // still shared copy-on-write and has to be made its own first (such storage
+  // has a context other than its memory).
+  void* data(Impl* x) const {
+    if (x->has_storage()) {
+      const at::DataPtr& p =
+          x->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks();
+      if (p.get() && (p.get() == p.get_context() || !c10::impl::cow::is_cow_data_ptr(p)))
+        return static_cast<char*>(p.get()) + x->storage_offset() * bytes;
+    }
+    return x->mutable_data();  // or an error that says why there is none
   }
 };
 
@@ -125,15 +139,6 @@ bool same_shape(const Impl* a, const Impl* b) {
 // `contiguous` says whether b is contiguous.
 bool same_layout(const Impl* a, const Impl* b, bool contiguous) {
   return (contiguous && a->is_contiguous()) || a->strides() == b->strides();
-}
-
-// The tensor's memory (an elements-less tensor has none): the storage's pointer
-// itself, unless it is still shared copy-on-write and has to be made its own.
-void* data_of(Impl* x) {
-  if (!x->has_storage()) return x->mutable_data();  // which says why there is none
-  const at::DataPtr& p = x->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks();
-  if (!p.get() || c10::impl::cow::is_cow_data_ptr(p)) return x->mutable_data();
-  return static_cast<char*>(p.get()) + x->storage_offset() * x->itemsize();
 }
 
 void check_like(const Impl* x, const Impl* p, bool contiguous, const TensorList& l,
@@ -254,6 +259,8 @@ std::optional<Tensor> advance(const Groups& r, uint32_t seed, const at::Device& 
   return coef;
 }
 
+// The tensor counts as changed from here on (a call that is refused later has
+// changed nothing, which a higher version does not hurt).
 void written_impl(Impl* x) {
   if (!x->is_inference()) x->bump_version();
 }
@@ -272,9 +279,10 @@ bool read_param(TensorList& params, TensorList& grads, Py_ssize_t i, const at::D
   s.dtype = dtype_code(p);
   s.numel = p->numel();
   if (!s.numel) return contiguous;
-  s.param = data_of(p);
+  written_impl(p);
+  s.param = params.data(p);
   if (same_layout(g, p, contiguous) && !g->is_neg()) {
-    s.grad = data_of(g);
+    s.grad = grads.data(g);
   } else {
     copies.push_back(at::empty_like(params[i]).copy_(grads[i]));
     s.grad = copies.back().data_ptr();
@@ -315,8 +323,8 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     check_like(mi, p, contiguous, m, i);
     check_like(vi, p, contiguous, v, i);
     if (!s.numel) continue;
-    written.add(s.exp_avg = data_of(mi), m, i);
-    written.add(s.exp_avg_sq = data_of(vi), v, i);
+    written.add(s.exp_avg = m.data(mi), m, i);
+    written.add(s.exp_avg_sq = v.data(vi), v, i);
   }
   set_groups(r, t);
   const std::optional<Tensor> coef = advance(r, 0, dev);
@@ -324,7 +332,6 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
                       coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
                       stream_of(dev)),
         "cs_adamw_step");
-  for (Py_ssize_t i = 0; i < params.n; ++i) written_impl(params[i].unsafeGetTensorImpl());
 }
 
 void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
@@ -357,10 +364,10 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
     check_scales(msi, scale_count(s.numel), ms, i);
     check_scales(vsi, scale_count(s.numel), vs, i);
     if (!s.numel) continue;
-    written.add(s.exp_avg = data_of(mi), m, i);
-    written.add(s.exp_avg_sq = data_of(vi), v, i);
-    written.add(s.exp_avg_scales = static_cast<uint8_t*>(data_of(msi)), ms, i);
-    written.add(s.exp_avg_sq_scales = static_cast<uint8_t*>(data_of(vsi)), vs, i);
+    written.add(s.exp_avg = m.data(mi), m, i);
+    written.add(s.exp_avg_sq = v.data(vi), v, i);
+    written.add(s.exp_avg_scales = static_cast<uint8_t*>(ms.data(msi)), ms, i);
+    written.add(s.exp_avg_sq_scales = static_cast<uint8_t*>(vs.data(vsi)), vs, i);
   }
   set_groups(r, t);
   const std::optional<Tensor> coef = advance(r, seed, dev);
@@ -368,7 +375,6 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
                        coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed, scale,
                        stream_of(dev)),
         "cs_adamw8_step");
-  for (Py_ssize_t i = 0; i < params.n; ++i) written_impl(params[i].unsafeGetTensorImpl());
 }
 
 void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
@@ -402,18 +408,16 @@ void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
     check_scales(msi, scale_count(s.numel), ms, i);
     check_scales(vsi, scale_count(s.numel), vs, i);
     if (!s.numel) continue;
-    s.exp_avg = data_of(c);
-    s.exp_avg_sq = data_of(vi);
-    s.exp_avg_scales = static_cast<uint8_t*>(data_of(msi));
-    s.exp_avg_sq_scales = static_cast<uint8_t*>(data_of(vsi));
-    written.add(s.param = data_of(omi), om, i);
-    written.add(s.grad = data_of(ovi), ov, i);
+    s.exp_avg = m.data(c);
+    s.exp_avg_sq = v.data(vi);
+    s.exp_avg_scales = static_cast<uint8_t*>(ms.data(msi));
+    s.exp_avg_sq_scales = static_cast<uint8_t*>(vs.data(vsi));
+    written_impl(omi);
+    written_impl(ovi);
+    written.add(s.param = om.data(omi), om, i);
+    written.add(s.grad = ov.data(ovi), ov, i);
   }
   check(cs_adamw8_moments(t.data(), (int32_t)t.size(), stream_of(dev)), "cs_adamw8_moments");
-  for (Py_ssize_t i = 0; i < m.n; ++i) {
-    written_impl(om[i].unsafeGetTensorImpl());
-    written_impl(ov[i].unsafeGetTensorImpl());
-  }
 }
 
 std::tuple<Tensor, Tensor> grad_norm(const py::object& grads_, double max_norm, double eps) {
@@ -432,7 +436,7 @@ std::tuple<Tensor, Tensor> grad_norm(const py::object& grads_, double max_norm, 
     t[i].numel = g->numel();
     if (!t[i].numel) continue;
     if (g->is_contiguous() || g->is_non_overlapping_and_dense()) {
-      t[i].data = data_of(g);
+      t[i].data = grads.data(g);
     } else {
       copies.push_back(grads[i].contiguous());
       t[i].data = copies.back().data_ptr();
