@@ -716,8 +716,11 @@ __global__ void adamw_advance_kernel(const __grid_constant__ AdvanceArgs a) {
 // ---------------------------------------------------------------------------
 // Global gradient norm: per-CTA sums in double in a fixed order, then one CTA.
 // Squares are formed in double, so neither 1e30 nor 1e-30 is lost.  403 M
-// bfloat16 elements take 123 us (6.54 TB/s, the copy rate; 150 us with the
-// conversion instruction and chunks of 16 KB), float32 227 us (7.1 TB/s).
+// bfloat16 elements take 122 us (6.6 TB/s, the copy rate; 150 us with the
+// conversion instruction and chunks of 16 KB), float32 227 us (7.1 TB/s).  Run
+// for a tenth of a second on end it meets the power limit (1.62 GHz, 138 us).
+// Squares in float32, which 16-bit types have exactly, and sums in double drew
+// less but took as long.
 
 struct NormEntry {
   const void* g;
@@ -760,39 +763,53 @@ __device__ __forceinline__ double block_sum_d(double v) {  // valid in thread 0
 
 // Sum of squares in double.  float32 is converted by the instruction for it.
 // That one runs at a quarter of the integer rate and bound the 16-bit types, so
-// theirs goes by integer operations: a float32's bits three places down in a
-// double's upper word (the low word is 0 for 11 significant bits) are |x|
-// 2^-896, subnormal numbers and zero included, and one exact product by 2^896
-// makes that |x|.  Infinities and NaN come out finite there, so the largest bits
-// are kept and looked at in the end.
+// theirs goes by integer operations, two elements a word: the exponent and
+// fraction bits moved to their places in a double's upper word are |x| times a
+// power of two (2^-896 for bfloat16, 2^-1008 for float16), subnormal numbers and
+// zero included, and one exact product makes that |x|.  Infinities and NaN come
+// out finite there, so the largest magnitude is kept and looked at in the end.
 template <class T>
-struct SquareSum {
+struct SquareSum;
+
+template <>
+struct SquareSum<float> {
+  using Bits = float;
   double acc = 0.0;
-  uint32_t most = 0;
-  __device__ __forceinline__ void add(float x) {
-    if (sizeof(T) == 4) {
-      acc = fma((double)x, (double)x, acc);
-    } else {
-      const uint32_t hi = (__float_as_uint(x) >> 3) & 0x0FFFFFFFu;
-      most = max(most, hi);
-      const double y = __hiloint2double((int)hi, 0) * 0x1p896;
-      acc = fma(y, y, acc);
-    }
-  }
-  __device__ __forceinline__ void add_words(const uint32_t (&w)[2 * sizeof(T)]) {
+  __device__ __forceinline__ void add(float x) { acc = fma((double)x, (double)x, acc); }
+  __device__ __forceinline__ void add_words(const uint32_t (&w)[8]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float2 x = unpack2<T>(w + u * (sizeof(T) / 2));
-      add(x.x);
-      add(x.y);
-    }
+    for (int u = 0; u < 8; ++u) add(__uint_as_float(w[u]));
+  }
+  __device__ __forceinline__ double sum() const { return acc; }
+};
+
+template <class Pair, int kLeft, int kRight, uint32_t kMask>
+struct SquareSum16 {
+  using Bits = uint16_t;
+  static constexpr double kFactor = kLeft == 13 ? 0x1p896 : 0x1p1008;
+  double lo = 0.0, hi = 0.0;
+  Pair most = {};
+  __device__ __forceinline__ void add_word(uint32_t w) {
+    most = __hmax2_nan(most, __habs2(*reinterpret_cast<Pair*>(&w)));
+    const double x = __hiloint2double((int)((w << kLeft) & kMask), 0) * kFactor;
+    const double y = __hiloint2double((int)((w >> kRight) & kMask), 0) * kFactor;
+    lo = fma(x, x, lo);
+    hi = fma(y, y, hi);
+  }
+  __device__ __forceinline__ void add(uint16_t x) { add_word(x); }
+  __device__ __forceinline__ void add_words(const uint32_t (&w)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add_word(w[u]);
   }
   __device__ __forceinline__ double sum() const {
-    constexpr uint32_t kInf = 0x7F800000u >> 3;
-    if (most < kInf) return acc;
-    return most == kInf ? __hiloint2double(0x7FF00000, 0) : __hiloint2double(0x7FF80000, 0);
+    const float m = to_f32(__hmax_nan(most.x, most.y));
+    return m < __int_as_float(0x7f800000) ? lo + hi : (double)m;
   }
 };
+template <>
+struct SquareSum<__nv_bfloat16> : SquareSum16<__nv_bfloat162, 13, 3, 0x0FFFE000u> {};
+template <>
+struct SquareSum<__half> : SquareSum16<__half2, 10, 6, 0x01FFFC00u> {};
 
 // A short or unaligned chunk, with as many loads at once.
 template <class T>
@@ -800,6 +817,8 @@ __device__ __noinline__ double norm_part(const T* g, int n, bool vec) {
   constexpr int kLoads = 16 / sizeof(T);
   const int thread = threadIdx.x % kNormThreads;
   SquareSum<T> s;
+  using Bits = typename SquareSum<T>::Bits;
+  const Bits* bits = reinterpret_cast<const Bits*>(g);
   if (vec) {  // all loads of the chunk at once, also of a short one
     uint32_t w[kLoads][2 * sizeof(T)];
 #pragma unroll
@@ -813,18 +832,18 @@ __device__ __noinline__ double norm_part(const T* g, int n, bool vec) {
       }
     }
     const int last = (n & ~7) + thread;
-    if (last < n) s.add(to_f32(g[last]));
+    if (last < n) s.add(bits[last]);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) s.add_words(w[u]);
     return s.sum();
   }
 #pragma unroll 1
   for (int from = thread; from < n; from += 8 * kNormThreads) {
-    float x[8];
+    Bits x[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = from + u * kNormThreads;
-      x[u] = i < n ? to_f32(g[i]) : 0.0f;
+      x[u] = i < n ? bits[i] : Bits(0);
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) s.add(x[u]);
@@ -858,10 +877,14 @@ template <int N>
 __device__ __forceinline__ double norm_chunks(const NormTable<N>& t) {
   const int groups = blockDim.x / kNormThreads;
   double acc = 0.0;
+  int k = 0, end = 0;  // the entry of the chunk before, and the chunk after its last
 #pragma unroll 1
   for (int c = blockIdx.x + gridDim.x * (threadIdx.x / kNormThreads); c < t.chunks;
        c += gridDim.x * groups) {
-    const int k = find_entry(t.first, t.count, c);
+    if (c >= end) {
+      k = find_entry(t.first, t.count, c);
+      end = k + 1 < t.count ? t.first[k + 1] : t.chunks;
+    }
     const NormEntry& e = t.e[k];
     const int chunk = c - t.first[k];
     const bool vec = (t.word[k] & 4) != 0;

@@ -14,7 +14,6 @@
  */
 #include <torch/extension.h>
 
-#include <c10/core/impl/COW.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -49,7 +48,8 @@ struct TensorList {
   PyObject** items;
   Py_ssize_t n;
   const char* name;
-  c10::DispatchKeySet keys;  // of the last tensor that passed all questions
+  PyTypeObject* kind = nullptr;  // Python type of the last tensor
+  c10::DispatchKeySet keys;      // of the last tensor that passed all questions
   caffe2::TypeMeta type;
   int64_t bytes = 0;  // of an element
   TensorList(const py::handle& seq, const char* what) : name(what) {
@@ -73,30 +73,39 @@ struct TensorList {
   // `takes` accepts (it names them otherwise).
   template <class Takes>
   Impl* get(Py_ssize_t i, const at::Device& dev, const Takes& takes) {
-    Impl* x = (*this)[i].unsafeGetTensorImpl();
-    if (x->key_set() == keys && x->dtype() == type && x->device() == dev) return x;
+    PyObject* o = items[i];
+    if (__builtin_expect(Py_TYPE(o) != kind, 0)) {
+      (*this)[i];
+      kind = Py_TYPE(o);
+    }
+    Impl* x = THPVariable_Unpack(o).unsafeGetTensorImpl();
+    if (__builtin_expect(x->key_set() == keys && x->dtype() == type && x->device() == dev, 1))
+      return x;
+    question(x, i, dev, takes(x->dtype().toScalarType()));
+    return x;
+  }
+  __attribute__((noinline)) void question(Impl* x, Py_ssize_t i, const at::Device& dev,
+                                          const char* want) {
     if (x->layout() != at::kStrided) bad(at(i) + " must be a dense tensor");
     if (!x->is_cuda()) bad(at(i) + " must be a CUDA tensor");
     if (x->device() != dev)
       bad(at(i) + " must be on " + dev.str() + ", got " + x->device().str());
-    if (const char* want = takes(x->dtype().toScalarType()))
+    if (want)
       bad(at(i) + " must be " + want + ", got " + c10::toString(x->dtype().toScalarType()));
+    if (!x->has_storage()) bad(at(i) + " must have a storage of its own");
     keys = x->key_set();
     type = x->dtype();
     bytes = (int64_t)type.itemsize();
-    return x;
   }
   // The memory of a tensor that get() returned: its storage's, unless that is
-  // still shared copy-on-write and has to be made its own first (such storage
-  // has a context other than its memory).
+  // still shared copy-on-write (it has a context other than its memory then) and
+  // has to be made its own first, or there is none, which is an error.
   void* data(Impl* x) const {
-    if (x->has_storage()) {
-      const at::DataPtr& p =
-          x->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks();
-      if (p.get() && (p.get() == p.get_context() || !c10::impl::cow::is_cow_data_ptr(p)))
-        return static_cast<char*>(p.get()) + x->storage_offset() * bytes;
-    }
-    return x->mutable_data();  // or an error that says why there is none
+    const at::DataPtr& p =
+        x->unsafe_storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks();
+    if (__builtin_expect(p.get() && p.get() == p.get_context(), 1))
+      return static_cast<char*>(p.get()) + x->storage_offset() * bytes;
+    return x->mutable_data();
   }
 };
 

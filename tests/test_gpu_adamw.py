@@ -85,6 +85,32 @@ def test_grad_norm_of_large_and_small_values():
             assert abs(float(scale) - c) <= 6.1e-8 * c
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_grad_norm_of_every_16_bit_value(dtype):
+    """All finite bit patterns (subnormal ones and zeros among them), alone in
+    their own tensors by magnitude, aligned and not; then each infinity and NaN."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).cuda()
+    every = bits.view(dtype)
+    finite = every[torch.isfinite(every)]
+    size = finite.float().abs()
+    small = torch.finfo(dtype).tiny
+    for g in (finite, finite[size < small], finite[size == 0], finite[size >= small][1:],
+              finite[size < small][3:]):
+        want, _ = oa.norm64([n64(g)])
+        norm, _ = ops.grad_norm([g])
+        if want > np.finfo(np.float32).max:  # rounds to infinity
+            assert torch.isinf(norm)
+            continue
+        # a norm below float32's normal range is rounded to its subnormal spacing
+        assert abs(float(norm) - want) <= 6.1e-8 * want + 2.0 ** -150
+    for at in (0, 1, 4099):
+        for bad in every[~torch.isfinite(every)][:: 9 if dtype == F16 else 1].tolist():
+            g = torch.ones(4100, dtype=dtype, device="cuda")
+            g[at] = bad
+            norm, _ = ops.grad_norm([g])
+            assert torch.isnan(norm) if bad != bad else torch.isinf(norm)
+
+
 def test_grad_norm_of_nan_inf_and_nothing():
     g = torch.ones(300, device="cuda")
     g[299] = float("nan")
