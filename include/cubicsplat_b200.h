@@ -424,8 +424,8 @@ CS_API int cs_adamw_step(const cs_adamw_tensor *tensors, int32_t count,
 /* The same step with moments of one byte an element and one scale byte E for
  * each block of 256: m is a sign, 4 exponent and 3 fraction bits, v 5 exponent
  * and 3 fraction bits, both with gradual underflow, in units of 2^(E-127);
- * E = 255 marks a block that is not finite.  Zeroed bytes stand for zero.  The
- * bytes are rounded stochastically from a hash of (seed, t, place of the tensor
+ * E = 255 marks a block that is not finite.  Zeroed bytes stand for zero.  An eps
+ * below 2^-60, the root of the smallest v, counts as 2^-60.  The bytes are rounded stochastically from a hash of (seed, t, place of the tensor
  * in the array, element), so a call is reproducible. */
 CS_API int cs_adamw8_step(const cs_adamw_tensor *tensors, int32_t count,
                    const cs_adamw_group *groups, int32_t num_groups, const float *coef,

@@ -68,8 +68,10 @@ def adamw8_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     2^-30 (v) of its block's largest.  They are rounded stochastically, by a
     hash of ``seed``, the step, the tensor's place in the list and the element,
     so an average moves by less than a code's width without being lost, and a
-    call is reproducible.  The step itself uses the moments before rounding.  A
-    block with a moment that is not finite (or above 1.5e38) turns NaN.
+    call is reproducible.  The step itself uses the moments before rounding, the
+    hardware's approximate square root and reciprocal (2^-22 each), and 2^-60, the
+    root of the smallest v, for a smaller ``eps``.  A block with a moment that is
+    not finite (or above 1.5e38) turns NaN.
     """
     _ext.load().adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs,
                             exp_avg_sq_scales,

@@ -284,7 +284,13 @@ class AdamW(Optimizer):
 
     def load_state_dict(self, state_dict):
         """As the base class, except that moments keep their own types (the base
-        class casts them to the parameter's) and are copies of the given ones."""
+        class casts them to the parameter's) and are copies of the given ones.
+        States of ``torch.optim.AdamW`` load too; what this class does not compute
+        (``maximize``, ``amsgrad``, Adam's coupled decay) is refused."""
+        for group in state_dict["param_groups"]:
+            if (group.get("maximize") or group.get("amsgrad")
+                    or not group.get("decoupled_weight_decay", True)):
+                raise ValueError("AdamW does not support maximize, amsgrad or coupled weight decay")
         super().load_state_dict({**state_dict, "state": {}})
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         own = [(p, g) for g in self.param_groups for p in g["params"]]

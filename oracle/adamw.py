@@ -65,10 +65,10 @@ def mix(h):
     return h ^ (h >> np.uint64(16))
 
 
-def random_bits(seed, step, place, numel):
-    """The 32 bits of every element, as uint32 [numel]."""
+def random_bits(seed, step, place, numel, first_block=0):
+    """The 32 bits of every element from a block on, as uint32 [numel]."""
     key = int(mix((seed + (step & 0xFFFFFFFF) * 0x9E3779B1) & 0xFFFFFFFF))
-    block = np.arange(-(-numel // BLOCK), dtype=np.uint64)
+    block = np.arange(-(-numel // BLOCK), dtype=np.uint64) + np.uint64(first_block)
     start = (key + place * 0x3C6EF373) & 0xFFFFFFFF
     b = mix((start + block * np.uint64(0xA54FF53B)) & 0xFFFFFFFF)
     h = (b[:, None] + np.arange(BLOCK, dtype=np.uint64) * np.uint64(0x9E3779B1)) & 0xFFFFFFFF
@@ -130,7 +130,7 @@ def decode_v(code, scales):
 
 
 def step8(g, m_codes, m_scales, v_codes, v_scales, *, step, betas=(0.9, 0.999), scale=None,
-          seed=0, place=0):
+          seed=0, place=0, first_block=0):
     """The moments' part of an 8-bit step: (m, v, m codes, m scales, v codes, v
     scales), m and v the float32 averages before rounding, everything flat."""
     b1, b2 = betas
@@ -141,7 +141,7 @@ def step8(g, m_codes, m_scales, v_codes, v_scales, *, step, betas=(0.9, 0.999), 
         m = (decode_m(m_codes, m_scales) * F32(b1)).astype(F32) + (g * F32(1 - b1)).astype(F32)
         v = (decode_v(v_codes, v_scales) * F32(b2)).astype(F32) \
             + ((g * g).astype(F32) * F32(1 - b2)).astype(F32)
-    bits = random_bits(seed, step, place, g.size)
+    bits = random_bits(seed, step, place, g.size, first_block)
     mc, me = encode_m(m, bits & U32(0xFFFF))
     vc, ve = encode_v(v, bits >> U32(16))
     return m.astype(F32), v.astype(F32), mc, me, vc, ve

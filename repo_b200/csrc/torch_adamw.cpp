@@ -268,16 +268,18 @@ std::optional<Tensor> advance(const Groups& r, uint32_t seed, const at::Device& 
   return coef;
 }
 
-// The tensor counts as changed from here on (a call that is refused later has
-// changed nothing, which a higher version does not hurt).
-void written_impl(Impl* x) {
-  if (!x->is_inference()) x->bump_version();
+// Tensors that a call has written: their versions go up once it is enqueued, so
+// that a graph which saved them notices.
+void bump_versions(const std::vector<Impl*>& changed) {
+  for (Impl* x : changed)
+    if (!x->is_inference()) x->bump_version();
 }
 
 // A parameter and its gradient; a gradient of another layout is copied.
 // Returns whether the parameter is contiguous.
 bool read_param(TensorList& params, TensorList& grads, Py_ssize_t i, const at::Device& dev,
-                cs_adamw_tensor& s, Impl*& p, std::vector<Tensor>& copies, Written& written) {
+                cs_adamw_tensor& s, Impl*& p, std::vector<Tensor>& copies,
+                std::vector<Impl*>& changed, Written& written) {
   p = params.get(i, dev, takes_float);
   const bool contiguous = p->is_contiguous();
   if (!contiguous && !p->is_non_overlapping_and_dense())
@@ -288,7 +290,7 @@ bool read_param(TensorList& params, TensorList& grads, Py_ssize_t i, const at::D
   s.dtype = dtype_code(p);
   s.numel = p->numel();
   if (!s.numel) return contiguous;
-  written_impl(p);
+  changed.push_back(p);
   s.param = params.data(p);
   if (same_layout(g, p, contiguous) && !g->is_neg()) {
     s.grad = grads.data(g);
@@ -322,11 +324,13 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
+  std::vector<Impl*> changed;
+  changed.reserve(params.n);
   Written written(3 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
     Impl* p;
-    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, written);
+    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, changed, written);
     Impl* mi = m.get(i, dev, takes_float32);
     Impl* vi = v.get(i, dev, takes_float32);
     check_like(mi, p, contiguous, m, i);
@@ -341,6 +345,7 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
                       coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
                       stream_of(dev)),
         "cs_adamw_step");
+  bump_versions(changed);
 }
 
 void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
@@ -359,11 +364,13 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
   const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
+  std::vector<Impl*> changed;
+  changed.reserve(params.n);
   Written written(5 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
     Impl* p;
-    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, written);
+    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, changed, written);
     Impl* mi = m.get(i, dev, takes_byte);
     Impl* vi = v.get(i, dev, takes_byte);
     check_like(mi, p, contiguous, m, i);
@@ -384,6 +391,7 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
                        coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed, scale,
                        stream_of(dev)),
         "cs_adamw8_step");
+  bump_versions(changed);
 }
 
 void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
@@ -397,6 +405,8 @@ void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
   const at::Device dev = device_of(m);
   c10::cuda::CUDAGuard guard(dev);
   std::vector<cs_adamw_tensor> t(m.n, cs_adamw_tensor{});
+  std::vector<Impl*> changed;
+  changed.reserve(2 * m.n);
   Written written(2 * m.n);
   for (Py_ssize_t i = 0; i < m.n; ++i) {
     cs_adamw_tensor& s = t[i];
@@ -421,12 +431,13 @@ void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
     s.exp_avg_sq = v.data(vi);
     s.exp_avg_scales = static_cast<uint8_t*>(ms.data(msi));
     s.exp_avg_sq_scales = static_cast<uint8_t*>(vs.data(vsi));
-    written_impl(omi);
-    written_impl(ovi);
+    changed.push_back(omi);
+    changed.push_back(ovi);
     written.add(s.param = om.data(omi), om, i);
     written.add(s.grad = ov.data(ovi), ov, i);
   }
   check(cs_adamw8_moments(t.data(), (int32_t)t.size(), stream_of(dev)), "cs_adamw8_moments");
+  bump_versions(changed);
 }
 
 std::tuple<Tensor, Tensor> grad_norm(const py::object& grads_, double max_norm, double eps) {

@@ -413,7 +413,7 @@ def test_offsets_past_32_bits():
     if torch.cuda.mem_get_info()[0] < 60 << 30:
         pytest.skip("needs 60 GB of free device memory")
     start = n - tail
-    assert start % 256 == 0
+    assert start % 256 == 0 and start < 1 << 31
     gen = torch.Generator().manual_seed(2)
     p = torch.zeros(n, dtype=BF16, device="cuda")
     g = torch.zeros(n, dtype=BF16, device="cuda")
@@ -431,8 +431,12 @@ def test_offsets_past_32_bits():
     np.testing.assert_array_equal(
         m[0][start:].cpu().numpy(),
         oa.decode_m(st[0][start:].cpu().numpy(), st[1][start // 256:].cpu().numpy()))
-    gap = np.abs(ref[1]) / 8 + np.abs(ref[1]).max() * 2.0 ** -16
-    assert (np.abs(n64(m[0][start:]) - ref[1]) <= gap).all()
+    zeros, scales = np.zeros(tail, np.uint8), np.zeros(4, np.uint8)
+    new = oa.step8(g[start:].float().cpu().numpy(), zeros, scales, zeros, scales, step=1,
+                   betas=HYPER["betas"], seed=3, first_block=start // 256)
+    for got, want in zip((st[0][start:], st[1][start // 256:], st[2][start:], st[3][start // 256:]),
+                         new[2:]):
+        np.testing.assert_array_equal(got.cpu().numpy(), want)
     del st
     m[0].zero_()
     v[0].zero_()
@@ -441,6 +445,66 @@ def test_offsets_past_32_bits():
     check_param(p[start:], BF16, ref[0], ref[3][0])
     assert (np.abs(n64(m[0][start:]) - ref[1]) <= ref[3][1]).all()
     assert not m[0][:start].any() and not p[:start].any()
+
+
+@pytest.mark.parametrize("dtype,n", [(F32, 5_000_077), (BF16, 20_000_300), (F16, 160_000_077)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_large_tensors_take_several_chunks_a_cta(shift, dtype, n):
+    """Sizes at which a CTA takes 2, 4 and 32 chunks, aligned and not, beside a
+    short tensor: windows of blocks at the start, around the CTAs' strides, in the
+    middle and at the cut end, against the restatement."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    p = (torch.randn(n + shift, device="cuda", generator=gen) * 0.3).to(dtype)[shift:]
+    g = (torch.randn(n + shift, device="cuda", generator=gen) * 1e-2).to(dtype)[shift:]
+    small = torch.zeros(70, device="cuda")
+    st, st2 = ops.adamw8_state(p), ops.adamw8_state(small)
+    ops.adamw8_step([small, p], [small + 1, g], *zip(st2, st), step=1, seed=3, **HYPER)
+    chunks = -(-n // 2048)
+    blocks = -(-n // 256)
+    starts = {0, blocks - 3, blocks // 2}
+    for per in (2, 4, 8, 16, 32):
+        stride = -(-chunks // per) * 8
+        starts |= {b for b in (stride - 2, stride * (per - 1) - 1) if 0 <= b < blocks - 3}
+    for b in sorted(starts):
+        at, end = b * 256, min(n, (b + 3) * 256)
+        zeros, scales = np.zeros(end - at, np.uint8), np.zeros(-(-(end - at) // 256), np.uint8)
+        gs = g[at:end].float().cpu().numpy()
+        new = oa.step8(gs, zeros, scales, zeros, scales, step=1, betas=HYPER["betas"], seed=3,
+                       place=1, first_block=b)
+        for got, want in zip((st[0][at:end], st[1][b:b + 3], st[2][at:end], st[3][b:b + 3]),
+                             new[2:]):
+            np.testing.assert_array_equal(got.cpu().numpy(), want)
+    # what is left of the whole: no element was skipped or moved twice
+    assert int((st[0] == 0).sum()) < n // 1000 and not (st[1] == 0).any()
+    m, v = moments_zero(p), moments_zero(p)
+    q = p.clone()
+    p2 = torch.empty(n + shift, dtype=dtype, device="cuda")[shift:]
+    p2.copy_(p)
+    ops.adamw_step([q], [g.clone()], [m], [v], step=1, **HYPER)
+    m2, v2 = moments_zero(p), moments_zero(p)
+    ops.adamw_step([small, p2], [small, g], [moments_zero(small), m2], [moments_zero(small), v2],
+                   step=1, **HYPER)
+    assert torch.equal(q, p2) and torch.equal(m, m2) and torch.equal(v, v2)
+    err = (m.double() - 0.1 * g.double()).abs() - 1e-6 * g.double().abs()
+    assert bool((err <= 1e-44).all())
+
+
+def moments_zero(p):
+    return torch.zeros(p.numel(), dtype=F32, device="cuda")
+
+
+def test_scalars_inference_tensors_and_tuples():
+    gen = torch.Generator().manual_seed(8)
+    s = make(1, F32, gen).view(())
+    st = ops.adamw8_state(s)
+    step8_and_check([s], [s.clone()], [st], 1)
+    with torch.inference_mode():
+        p, g = make(700, F32, gen), make(700, F32, gen)
+        m, v = moments32(p, gen)
+        want = oa.adamw64(n64(p), n64(g), n64(m), n64(v), 2, **HYPER)
+        norm, scale = ops.grad_norm((g,))
+        ops.adamw_step((p,), (g,), (m,), (v,), step=2, **HYPER)
+        check_param(p, F32, want[0], want[3][0])
 
 
 # --- refusals ---------------------------------------------------------------
@@ -486,6 +550,7 @@ def test_refusals():
     with pytest.raises(ValueError, match="out\\[0\\]\\[0\\] must be Float"):
         ops.adamw8_moments([c], [s], [c], [s], out=([c], [t()]))
     assert not p.any() and not m.any() and not v.any() and not c.any() and not s.any()
+    assert p._version == 0  # a refused call has changed nothing
 
 
 # --- optimiser --------------------------------------------------------------
@@ -669,6 +734,30 @@ def test_state_dict_round_trip(bits, capturable):
         with pytest.raises(ValueError, match="state_bits"):
             other.param_groups[0]["state_bits"] = 32
             other.step()
+
+
+def test_state_of_torch_adamw_loads_and_continues():
+    """Two steps of torch's AdamW, then one here from its state, against float64
+    from that state; what this class does not compute is refused."""
+    gen = torch.Generator().manual_seed(3)
+    p = make(1000, F32, gen, 0.3).requires_grad_()
+    kw = dict(lr=1e-2, betas=(0.8, 0.99), weight_decay=0.1)
+    old = torch.optim.AdamW([p], **kw)
+    for _ in range(2):
+        p.grad = make(1000, F32, gen)
+        old.step()
+    opt = manbo.AdamW([p])
+    opt.load_state_dict(old.state_dict())
+    m, v = opt.moments(p)
+    p.grad = make(1000, F32, gen)
+    want = oa.adamw64(n64(p), n64(p.grad), n64(m), n64(v), 3, **kw)
+    opt.step()
+    check_param(p, F32, want[0], want[3][0])
+    assert opt.state[p]["step"] == 3
+    for other in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True),
+                  torch.optim.Adam([p])):
+        with pytest.raises(ValueError, match="does not support"):
+            opt.load_state_dict(other.state_dict())
 
 
 @pytest.mark.parametrize("bits", [8, 32])
