@@ -19,7 +19,7 @@
 
 namespace cs {
 
-constexpr int kChunkThreads = 256;
+constexpr int kChunkThreads = 128;
 constexpr int kPerThread = 8;
 constexpr int kBlock8 = CS_ADAMW8_BLOCK;                  // elements of a scale block: one warp's
 constexpr int kChunk = kChunkThreads * kPerThread;        // elements of a CTA's chunk
@@ -393,11 +393,12 @@ __device__ __noinline__ uint32_t raised_zeros(uint32_t w, float a, float b, floa
 // depend on it.  `first` is the element of the lane's first value in the block,
 // kStride the distance of the next.
 //
-// With 16-bit parameters the instructions bound it, not the memory: some 48 an
-// element, 20 of them integer.  268 M bfloat16 elements take 460 us (5.85 TB/s,
-// 89% of the copy rate; 618 us before the codes were built word by word, the
+// With 16-bit parameters the instructions bound it, not the memory: some 47 an
+// element, 20 of them integer.  268 M bfloat16 elements take 444 us (6.05 TB/s,
+// 93% of the copy rate; 618 us before the codes were built word by word, the
 // per-block values prepared a block a lane and the next block prefetched),
-// float32 657 us (6.54 TB/s, the copy rate).
+// float32 654 us (6.57 TB/s, the copy rate).  Seven CTAs of 128 threads an SM
+// leave 72 registers a thread, which just hold it; three of 256 took 459 us.
 template <int kStride>
 __device__ __forceinline__ void step_lane8(const StepCoef8& c, float2 (&P)[4],
                                            const float2 (&G)[4], uint32_t (&mw)[2],
@@ -575,8 +576,8 @@ __device__ __forceinline__ void step_part8(const AdamEntry8& e, const StepCoef8&
 // (neighbouring chunks for each CTA were 2.4 times slower: everything in flight
 // was a slice of 8 KB in every 64).  What a block has one of (scales, key) is
 // prepared and stored for all of the warp's blocks at once, a block a lane (32
-// blocks a warp at most; 268 M bfloat16 elements take 469 us so, 492 with eight,
-// 594 with two).
+// blocks a warp at most; with eight at most 268 M bfloat16 elements took 5%
+// longer, with two 27%).
 // With 16-bit parameters the next block's loads are issued before the present
 // one's arithmetic (they need 12 registers; float32's 20 would cost a CTA of
 // occupancy).
@@ -586,8 +587,8 @@ __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8&
   constexpr uint32_t kWarps = kChunkThreads / 32;
   const int lane = threadIdx.x & 31;
   const uint32_t chunks = (uint32_t)((e.numel + kChunk - 1) / kChunk);
-  const uint32_t stride = (chunks + (1u << shift) - 1) >> shift << 3;
-  static_assert(kWarps == 8, "3 bits");
+  const uint32_t stride = (chunks + (1u << shift) - 1) >> shift << 2;
+  static_assert(kWarps == 4, "2 bits");
   const uint32_t first = chunk * kWarps + (threadIdx.x >> 5);
   const uint32_t end = (uint32_t)((e.numel + kBlock8 - 1) / kBlock8);
   const uint32_t full = (e.word & 4) ? (uint32_t)(e.numel / kBlock8) : 0;
@@ -642,7 +643,7 @@ __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8&
 }
 
 template <int N>
-__global__ void __launch_bounds__(kChunkThreads, 3)
+__global__ void __launch_bounds__(kChunkThreads, 7)
     adamw8_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
@@ -811,42 +812,34 @@ struct SquareSum<__nv_bfloat16> : SquareSum16<__nv_bfloat162, 13, 3, 0x0FFFE000u
 template <>
 struct SquareSum<__half> : SquareSum16<__half2, 10, 6, 0x01FFFC00u> {};
 
-// A short or unaligned chunk, with as many loads at once.
+// A short or unaligned chunk: the elements before the first 16-byte border and
+// after the last one by themselves, the rest with half as many loads at once.
 template <class T>
-__device__ __noinline__ double norm_part(const T* g, int n, bool vec) {
-  constexpr int kLoads = 16 / sizeof(T);
+__device__ __noinline__ double norm_part(const T* g, int n) {
+  constexpr int kLoads = 16 / sizeof(T), kWords = 2 * sizeof(T);
   const int thread = threadIdx.x % kNormThreads;
   SquareSum<T> s;
   using Bits = typename SquareSum<T>::Bits;
+  const int head = min(n, (int)((-reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T)));
   const Bits* bits = reinterpret_cast<const Bits*>(g);
-  if (vec) {  // all loads of the chunk at once, also of a short one
-    uint32_t w[kLoads][2 * sizeof(T)];
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int i = (u * kNormThreads + thread) * 8;
-      if (i + 8 <= n) {
-        load_words(reinterpret_cast<const char*>(g + i), w[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2 * (int)sizeof(T); ++j) w[u][j] = 0;
-      }
-    }
-    const int last = (n & ~7) + thread;
-    if (last < n) s.add(bits[last]);
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) s.add_words(w[u]);
-    return s.sum();
-  }
+  if (thread < head) s.add(bits[thread]);
+  g += head;
+  bits += head;
+  n -= head;
+  const int last = (n & ~7) + thread;
+  if (last < n) s.add(bits[last]);
 #pragma unroll 1
-  for (int from = thread; from < n; from += 8 * kNormThreads) {
-    Bits x[8];
+  for (int from = thread * 8; from + 8 <= n; from += kLoads / 2 * kNormThreads * 8) {
+    uint32_t w[kLoads / 2][kWords];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = from + u * kNormThreads;
-      x[u] = i < n ? bits[i] : Bits(0);
+    for (int u = 0; u < kLoads / 2; ++u) {
+      const int i = from + u * kNormThreads * 8;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) w[u][j] = 0;
+      if (i + 8 <= n) load_words(reinterpret_cast<const char*>(g + i), w[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s.add(x[u]);
+    for (int u = 0; u < kLoads / 2; ++u) s.add_words(w[u]);
   }
   return s.sum();
 }
@@ -861,7 +854,7 @@ __device__ __forceinline__ double norm_chunk(const void* data, int chunk, int64_
   const T* g = static_cast<const T*>(data) + at;
   const int64_t left = numel - at;
   const int n = left < kElems ? (int)left : kElems;
-  if (!vec || n < kElems) return norm_part(g, n, vec);
+  if (!vec || n < kElems) return norm_part(g, n);
   SquareSum<T> s;
   uint32_t w[kLoads][2 * sizeof(T)];
 #pragma unroll
@@ -992,7 +985,9 @@ struct GroupBuilder {
 // `width` bytes.
 inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
                        AdamEntry& e) {
-  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq) return false;
+  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !aligned_to(s.exp_avg, 4) ||
+      !aligned_to(s.exp_avg_sq, 4))
+    return false;
   const int64_t bytes = at * dtype_size(s.dtype);
   e.p = static_cast<char*>(s.param) + bytes;
   e.g = static_cast<const char*>(s.grad) + bytes;
@@ -1026,11 +1021,15 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t a
   return true;
 }
 
-// A CTA takes several chunks (a power of two) where enough CTAs are left: eight
-// an SM for two chunks, 16 for more.  Measured with 8-bit moments: 7 M elements
-// in 300 tensors 22 us with one chunk, 18 with two; 33 M float32 elements 87 us
-// with four, 95 with 16.
-constexpr int64_t ctas_wanted(int shift) { return shift == 1 ? 148 * 8 : 148 * 16; }
+// A CTA takes several chunks (a power of two) where enough CTAs are left an SM:
+// eight for two chunks and 16 for more, or 56 where all parameters are float32,
+// whose next block is not prefetched, so that only the end of the launch counts.
+// Measured with 8-bit moments: 7 M elements in 300 tensors of all types 22 us
+// with one chunk, 18 with two; 33 M bfloat16 elements 31 us with 16 CTAs an SM,
+// 37 with 56; 150 M float32 elements 372 and 358 us.
+constexpr int64_t ctas_wanted(int shift, bool half) {
+  return 148 * (shift == 1 ? 8 : half ? 16 : 56);
+}
 
 // The kernels of one table type, by name.
 struct RunStep {
@@ -1065,12 +1064,18 @@ int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const A
   t.grad_scale = grad_scale;
   for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
   int64_t total = 0;
-  for (int i = 0; i < count; ++i) total += (tensors[i].numel + kChunk - 1) / kChunk;
+  bool half = false;
+  for (int i = 0; i < count; ++i) {
+    total += (tensors[i].numel + kChunk - 1) / kChunk;
+    half |= tensors[i].dtype != CS_F32;
+  }
   int shift = 0;
-  while ((1 << shift) < Run::kMostPer && (total >> (shift + 1)) >= ctas_wanted(shift + 1)) ++shift;
+  while ((1 << shift) < Run::kMostPer &&
+         (total >> (shift + 1)) >= ctas_wanted(shift + 1, half))
+    ++shift;
   t.shift = shift;
-  static_assert(kChunk == 2048, "11 bits");
-  shift += 11;
+  static_assert(kChunk == 1024, "10 bits");
+  shift += 10;
   t.count = 0;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
@@ -1101,6 +1106,8 @@ inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups) 
     if (s.numel < 0 || s.numel > kMaxNumel || s.dtype < CS_F32 || s.dtype > CS_F16 ||
         s.group < 0 || s.group >= groups)
       return CS_ERR_ARG;
+    const int size = dtype_size(s.dtype);
+    if (!aligned_to(s.param, size) || !aligned_to(s.grad, size)) return CS_ERR_ARG;
   }
   return CS_OK;
 }
@@ -1265,7 +1272,8 @@ int cs_grad_norm(const cs_grad_tensor* tensors, int32_t count, double max_norm, 
     return CS_ERR_ARG;
   for (int i = 0; i < count; ++i)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || tensors[i].dtype < CS_F32 ||
-        tensors[i].dtype > CS_F16 || (tensors[i].numel > 0 && !tensors[i].data))
+        tensors[i].dtype > CS_F16 || (tensors[i].numel > 0 && !tensors[i].data) ||
+        !aligned_to(tensors[i].data, dtype_size(tensors[i].dtype)))
       return CS_ERR_ARG;
   cudaStream_t st = (cudaStream_t)stream;
   const NormOut out{max_norm, eps, norm, scale};

@@ -55,7 +55,8 @@ def _step(name, tensor, group=None, count=1, groups=1):
 def test_c_entries_refuse_bad_tables(name):
     for bad in (dict(numel=-1), dict(numel=(1 << 40) + 1), dict(dtype=3), dict(dtype=-1),
                 dict(group=1), dict(group=-1), dict(param=None), dict(grad=None),
-                dict(exp_avg=None), dict(exp_avg_sq=None)):
+                dict(exp_avg=None), dict(exp_avg_sq=None), dict(param=258),
+                dict(grad=513, dtype=1)):
         assert _step(name, _tensor(**bad)) == CS_ERR_ARG, bad
     for bad in (dict(beta1=1.0), dict(beta2=1.0), dict(beta1=-0.1), dict(beta2=float("nan")),
                 dict(step=0)):
@@ -90,7 +91,9 @@ def test_c_entries_refuse_missing_scales_counters_and_workspaces():
     for args in ((at, -1, 64, 64, 64), (None, 1, 64, 64, 64), (at, 1, None, 64, 64),
                  (at, 1, 64, 64, None), (at, 1, 64, 64, 68)):
         assert nat.call("cs_grad_norm", args[0], args[1], 1.0, 1e-6, *args[2:], None) == CS_ERR_ARG
-    for bad in (CGrad(None, 4, 0, 0), CGrad(256, -4, 0, 0), CGrad(256, 4, 9, 0)):
+    assert _step("cs_adamw_step", _tensor(exp_avg=1026)) == CS_ERR_ARG
+    for bad in (CGrad(None, 4, 0, 0), CGrad(256, -4, 0, 0), CGrad(256, 4, 9, 0),
+                CGrad(258, 4, 0, 0), CGrad(257, 4, 1, 0)):
         n = (CGrad * 1)(bad)
         assert nat.call("cs_grad_norm", ctypes.addressof(n), 1, 1.0, 1e-6, 64, 64, 64,
                         None) == CS_ERR_ARG

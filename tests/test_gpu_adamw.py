@@ -450,7 +450,7 @@ def test_offsets_past_32_bits():
 @pytest.mark.parametrize("dtype,n", [(F32, 5_000_077), (BF16, 20_000_300), (F16, 160_000_077)])
 @pytest.mark.parametrize("shift", [0, 1])
 def test_large_tensors_take_several_chunks_a_cta(shift, dtype, n):
-    """Sizes at which a CTA takes 2, 4 and 32 chunks, aligned and not, beside a
+    """Sizes at which a CTA takes several chunks (up to 32), aligned and not, beside a
     short tensor: windows of blocks at the start, around the CTAs' strides, in the
     middle and at the cut end, against the restatement."""
     gen = torch.Generator(device="cuda").manual_seed(n)
@@ -459,11 +459,11 @@ def test_large_tensors_take_several_chunks_a_cta(shift, dtype, n):
     small = torch.zeros(70, device="cuda")
     st, st2 = ops.adamw8_state(p), ops.adamw8_state(small)
     ops.adamw8_step([small, p], [small + 1, g], *zip(st2, st), step=1, seed=3, **HYPER)
-    chunks = -(-n // 2048)
+    chunks = -(-n // 1024)  # four scale blocks
     blocks = -(-n // 256)
     starts = {0, blocks - 3, blocks // 2}
     for per in (2, 4, 8, 16, 32):
-        stride = -(-chunks // per) * 8
+        stride = -(-chunks // per) * 4
         starts |= {b for b in (stride - 2, stride * (per - 1) - 1) if 0 <= b < blocks - 3}
     for b in sorted(starts):
         at, end = b * 256, min(n, (b + 3) * 256)
