@@ -270,7 +270,9 @@ class AdamW(Optimizer):
     @torch.no_grad()
     def moments(self, p):
         """(exp_avg, exp_avg_sq) of a parameter as new float32 tensors."""
-        st = self.state[p]
+        st = self.state.get(p)
+        if not st:
+            raise ValueError("the parameter has no state yet: it has not taken a step")
         if "exp_avg_scales" not in st:
             return st["exp_avg"].clone(), st["exp_avg_sq"].clone()
         m, v = adamw8_moments([st["exp_avg"]], [st["exp_avg_scales"]], [st["exp_avg_sq"]],

@@ -8,8 +8,9 @@
 // one launch covers all tensors of a call up to the table's capacity.  A CTA
 // finds the tensor of its chunk by a binary search over the chunk prefix.
 //
-// All of it is bound by HBM: the step moves 28 B an element (float32) or 22 B
-// (16-bit parameters), with 8-bit moments 16 B or 10 B.
+// The step moves 28 B an element (float32) or 22 B (16-bit parameters) and is
+// bound by HBM: 268 M float32 elements take 1.08 ms (6.97 TB/s), bfloat16 ones
+// 0.85 ms.  With 8-bit moments it moves 16 B or 10 B.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -38,28 +39,29 @@ struct AdamGroup {
   const float* coef;                                  // {ibc1, rbc2, key bits} where given
 };
 
-struct AdamEntry {  // m, v: float moments, or codes with their scale bytes
+struct AdamEntry {
   void* p;
   const void* g;
   void* m;
   void* v;
   int64_t numel;
-  uint32_t word;  // dtype 0-1, vector path 2, group 3-7, place 8-31... (see entry_word)
+  uint32_t word;  // see entry_word
   uint32_t pad;
 };
 
 struct AdamEntry8 {
   void* p;
   const void* g;
-  uint8_t* m;
+  uint8_t* m;   // codes
   uint8_t* v;
-  uint8_t* ms;
+  uint8_t* ms;  // scale bytes
   uint8_t* vs;
   int64_t numel;
   uint32_t word;
   uint32_t block0;  // number of its first block in its tensor
 };
 
+// Bits 0-1 type, 2 vector path, 3-7 group, 8-31 place in the call's array.
 constexpr uint32_t entry_word(int dtype, bool vec, int group, int place) {
   return (uint32_t)dtype | (vec ? 4u : 0u) | ((uint32_t)group << 3) | ((uint32_t)place << 8);
 }
@@ -109,7 +111,7 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
 template <class T>
-struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) Pack8 {
+struct alignas(16) Pack8 {
   T x[8];
 };
 
@@ -127,12 +129,6 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<Pack8<T>*>(p) = q;
 }
 
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float2 (&x)[4]) {
-  const Pack8<T> q = *reinterpret_cast<const Pack8<T>*>(p);
-#pragma unroll
-  for (int u = 0; u < 4; ++u) x[u] = make_float2(to_f32(q.x[2 * u]), to_f32(q.x[2 * u + 1]));
-}
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float2 (&x)[4]) {
   Pack8<T> q;
@@ -179,8 +175,8 @@ __device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* g
   return c;
 }
 
-// One element.  The moments' arithmetic is one rounding an operation in the
-// order written; the 8-bit moments' bytes are defined by it.
+// One element, in float32 with one rounding an operation in the order written
+// (step_lane8 does the same to m and v, whose bytes are defined by it).
 __device__ __forceinline__ void adamw_element(const StepCoef& c, float& p, float g, float& m,
                                               float& v) {
   g = g * c.scale;
@@ -397,7 +393,7 @@ __device__ __noinline__ uint32_t raised_zeros(uint32_t w, float a, float b, floa
 // element, 20 of them integer.  268 M bfloat16 elements take 444 us (6.05 TB/s,
 // 93% of the copy rate; 618 us before the codes were built word by word, the
 // per-block values prepared a block a lane and the next block prefetched),
-// float32 654 us (6.57 TB/s, the copy rate).  Seven CTAs of 128 threads an SM
+// float32 643 us (6.68 TB/s, the copy rate).  Seven CTAs of 128 threads an SM
 // leave 72 registers a thread, which just hold it; three of 256 took 459 us.
 template <int kStride>
 __device__ __forceinline__ void step_lane8(const StepCoef8& c, float2 (&P)[4],
@@ -579,8 +575,8 @@ __device__ __forceinline__ void step_part8(const AdamEntry8& e, const StepCoef8&
 // blocks a warp at most; with eight at most 268 M bfloat16 elements took 5%
 // longer, with two 27%).
 // With 16-bit parameters the next block's loads are issued before the present
-// one's arithmetic (they need 12 registers; float32's 20 would cost a CTA of
-// occupancy).
+// one's arithmetic (they need 12 registers; float32's 20 spill at seven CTAs an
+// SM, 698 us for 268 M elements instead of 643, and gain nothing at five).
 template <class T>
 __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8& c, uint32_t chunk,
                                            int shift) {
@@ -918,7 +914,10 @@ template <int N>
 __global__ void __launch_bounds__(kNormThreads * kNormGroups)
     grad_norm_small_kernel(const __grid_constant__ NormTable<N> t, NormOut out) {
   __shared__ double sums[kNormCluster];
+  // the first CTA has to have started before another one writes to it
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   const double acc = norm_chunks(t);
+  asm volatile("barrier.cluster.wait;" ::: "memory");
   if (threadIdx.x == 0) {
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(sums + blockIdx.x);
     uint32_t first;
