@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "cs_common.cuh"
 
@@ -713,11 +714,9 @@ __global__ void adamw_advance_kernel(const __grid_constant__ AdvanceArgs a) {
 // ---------------------------------------------------------------------------
 // Global gradient norm: per-CTA sums in double in a fixed order, then one CTA.
 // Squares are formed in double, so neither 1e30 nor 1e-30 is lost.  403 M
-// bfloat16 elements take 122 us (6.6 TB/s, the copy rate; 150 us with the
-// conversion instruction and chunks of 16 KB), float32 227 us (7.1 TB/s).  Run
-// for a tenth of a second on end it meets the power limit (1.62 GHz, 138 us).
-// Squares in float32, which 16-bit types have exactly, and sums in double drew
-// less but took as long.
+// bfloat16 elements take 120 us (6.7 TB/s, the copy rate; 150 us with the
+// conversion instruction and chunks of 16 KB), float32 228 us (7.0 TB/s).  Run
+// for a tenth of a second on end it meets the power limit.
 
 struct NormEntry {
   const void* g;
@@ -840,6 +839,14 @@ __device__ __noinline__ double norm_part(const T* g, int n) {
   return s.sum();
 }
 
+// A square p as float32 times 2^-896: its bits three places down in a double
+// (kLow: with more than 20 fraction bits, which the upper word does not hold).
+template <bool kLow>
+__device__ __forceinline__ double square_bits(float p) {
+  const uint32_t b = __float_as_uint(p);
+  return __hiloint2double((int)(b >> 3), kLow ? (int)(b << 29) : 0);
+}
+
 template <class T>
 __device__ __forceinline__ double norm_chunk(const void* data, int chunk, int64_t numel,
                                              bool vec) {
@@ -851,14 +858,38 @@ __device__ __forceinline__ double norm_chunk(const void* data, int chunk, int64_
   const int64_t left = numel - at;
   const int n = left < kElems ? (int)left : kElems;
   if (!vec || n < kElems) return norm_part(g, n);
-  SquareSum<T> s;
   uint32_t w[kLoads][2 * sizeof(T)];
 #pragma unroll
   for (int u = 0; u < kLoads; ++u)
     load_words(reinterpret_cast<const char*>(g + (u * kNormThreads + thread) * 8), w[u]);
+  if (sizeof(T) == 4) {
+    SquareSum<T> s;
 #pragma unroll
-  for (int u = 0; u < kLoads; ++u) s.add_words(w[u]);
-  return s.sum();
+    for (int u = 0; u < kLoads; ++u) s.add_words(w[u]);
+    return s.sum();
+  }
+  // Squares of 16-bit types are exact in float32 (16 and 22 significant bits)
+  // where they stay in its range, which leaves one addition in double: fewer
+  // operations, and less power (403 M bfloat16 elements on end: 121 us, 136 with
+  // the squares in double).  A sum that is not well inside the range is formed
+  // again by norm_part, which takes every value, unless all elements are zero.
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  double lo = 0.0, hi = 0.0;
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      any |= w[u][j];
+      const float2 x = unpack2<T>(&w[u][j]);
+      const float2 p = __fmul2_rn(x, x);
+      lo += square_bits<kHalf>(p.x);
+      hi += square_bits<kHalf>(p.y);
+    }
+  }
+  const double sum = (lo + hi) * 0x1p896;
+  const bool fine = (sum >= 0x1p-90 && sum < 0x1p120) || !(any & 0x7FFF7FFFu);
+  return __any_sync(0xffffffffu, !fine) ? norm_part(g, n) : sum;
 }
 
 // The CTA's chunks, one for each 256 of its threads at a time.

@@ -111,6 +111,34 @@ def test_grad_norm_of_every_16_bit_value(dtype):
             assert torch.isnan(norm) if bad != bad else torch.isinf(norm)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_grad_norm_of_full_chunks_of_every_size(dtype):
+    """Long aligned tensors: ordinary values, zeros, zeros with signs, and values
+    whose squares float32 does not hold, alone and among ordinary ones."""
+    gen = torch.Generator().manual_seed(2)
+    n = 1 << 18
+    ordinary = make(n, dtype, gen)
+    kinds = [ordinary, torch.zeros(n, dtype=dtype, device="cuda"),
+             -torch.zeros(n, dtype=dtype, device="cuda")]
+    for size in ((1e-6, 6e4) if dtype == F16 else (1e-39, 1e-25, 1e-16, 1e16, 1e25)):
+        some = ordinary.clone()
+        some[::1000] = size
+        kinds += [some, torch.full((n,), size, dtype=dtype, device="cuda"),
+                  torch.cat([ordinary[:n // 2], torch.full((n // 2,), size, dtype=dtype,
+                                                           device="cuda")])]
+    for g in kinds:
+        want, _ = oa.norm64([n64(g)])
+        norm, _ = ops.grad_norm([g, ordinary[:5]])
+        want = (want ** 2 + float((n64(ordinary[:5]) ** 2).sum())) ** 0.5
+        assert abs(float(norm) - want) <= 6.1e-8 * want
+    for at in (0, n - 1):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            g = ordinary.clone()
+            g[at] = bad
+            norm, _ = ops.grad_norm([g])
+            assert torch.isnan(norm) if bad != bad else torch.isinf(norm)
+
+
 def test_grad_norm_of_nan_inf_and_nothing():
     g = torch.ones(300, device="cuda")
     g[299] = float("nan")
