@@ -48,6 +48,7 @@ struct TensorList {
   PyObject** items;
   Py_ssize_t n;
   const char* name;
+  bool lazy = false;             // takes tensors whose sign is still to be applied
   PyTypeObject* kind = nullptr;  // Python type of the last tensor
   c10::DispatchKeySet keys;      // of the last tensor that passed all questions
   caffe2::TypeMeta type;
@@ -93,6 +94,7 @@ struct TensorList {
     if (want)
       bad(at(i) + " must be " + want + ", got " + c10::toString(x->dtype().toScalarType()));
     if (!x->has_storage()) bad(at(i) + " must have a storage of its own");
+    if (!lazy && x->is_neg()) bad(at(i) + " must not be a lazily negated view");
     keys = x->key_set();
     type = x->dtype();
     bytes = (int64_t)type.itemsize();
@@ -316,6 +318,7 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       v(exp_avg_sqs_, "exp_avg_sqs");
   for (const TensorList* l : {&grads, &m, &v}) same_length(params, *l);
+  grads.lazy = true;
   if (params.n == 0) return;
   const Groups r = read_groups(groups, params.n, params[0].device());
   const at::Device dev = device_of(params);
@@ -356,6 +359,7 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
       ms(m_scales_, "exp_avg_scales"), v(exp_avg_sqs_, "exp_avg_sqs"),
       vs(v_scales_, "exp_avg_sq_scales");
   for (const TensorList* l : {&grads, &m, &ms, &v, &vs}) same_length(params, *l);
+  grads.lazy = true;
   if (params.n == 0) return;
   const Groups r = read_groups(groups, params.n, params[0].device());
   const at::Device dev = device_of(params);
@@ -443,6 +447,7 @@ void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
 std::tuple<Tensor, Tensor> grad_norm(const py::object& grads_, double max_norm, double eps) {
   TensorList grads(grads_, "grads");
   if (grads.n == 0) bad("grads must not be empty");
+  grads.lazy = true;  // the norm of -x is that of x
   if (!(max_norm >= 0.0)) bad("Invalid max_norm: " + std::to_string(max_norm));
   if (!(eps >= 0.0)) bad("Invalid epsilon value: " + std::to_string(eps));
   const at::Device dev = device_of(grads);

@@ -236,7 +236,8 @@ def test_adamw_step_of_other_layouts():
     p = make(840, F32, gen).view(shape).contiguous(memory_format=torch.channels_last)
     m, v = moments32(p, gen)
     for g in (make(840, F32, gen).view(shape), make(1680, F32, gen).view(4, 6, 5, 14)[..., ::2],
-              make(1, F32, gen).expand(shape)):
+              make(1, F32, gen).expand(shape), torch._neg_view(p.clone(
+                  memory_format=torch.preserve_format))):
         want = oa.adamw64(n64(p), n64(g), n64(m), n64(v), 7, **HYPER)
         ops.adamw_step([p], [g], [m], [v], step=7, **HYPER)
         check_param(p, F32, want[0], want[3][0])
@@ -575,6 +576,10 @@ def test_refusals():
             (([p], [g], [c], [s], [c], [t(1, torch.uint8)]), "exp_avg_sqs\\[0\\] is given twice")):
         with pytest.raises(ValueError, match=msg):
             ops.adamw8_step(*args, step=1)
+    with pytest.raises(ValueError, match="params\\[0\\] must not be a lazily negated view"):
+        ops.adamw_step([torch._neg_view(p)], [g], [m], [v], step=1)
+    with pytest.raises(ValueError, match="exp_avgs\\[0\\] must not be a lazily negated view"):
+        ops.adamw_step([p], [g], [torch._neg_view(m)], [v], step=1)
     with pytest.raises(ValueError, match="out\\[0\\]\\[0\\] must be Float"):
         ops.adamw8_moments([c], [s], [c], [s], out=([c], [t()]))
     assert not p.any() and not m.any() and not v.any() and not c.any() and not s.any()
