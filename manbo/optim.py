@@ -199,19 +199,21 @@ class AdamW(Optimizer):
         return st
 
     def _plan(self):
-        """{(device, state_bits): [(group, step, parameters)]} of this step, the
-        parameters of an entry at the same step."""
+        """{(device index, state_bits, seed): [(group, step, parameters, gradients,
+        states)]} of this step, the parameters of an entry at the same step."""
         plan = {}
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for group in self.param_groups:
             cohorts, counters = {}, {}
-            if capturing and not group["capturable"]:
+            eight, capturable = group["state_bits"] == 8, bool(group["capturable"])
+            if capturing and not capturable:
                 raise RuntimeError("AdamW: a captured step needs capturable=True")
-            eight = group["state_bits"] == 8
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                if not p.is_cuda:
+                device = p.get_device()
+                if device < 0:
                     raise ValueError("AdamW parameters must be CUDA tensors")
                 st = self.state[p]
                 if not st:
@@ -219,13 +221,17 @@ class AdamW(Optimizer):
                 if ("exp_avg_scales" in st) != eight:
                     raise ValueError(f"AdamW state is not of state_bits={group['state_bits']}")
                 step = st["step"]
-                if isinstance(step, torch.Tensor) != bool(group["capturable"]):
+                if isinstance(step, torch.Tensor) != capturable:
                     raise ValueError("AdamW state was made with another value of capturable")
-                key = (p.device, id(step) if group["capturable"] else step)
-                if key not in cohorts:
-                    cohorts[key] = (group, step, [])
-                    plan.setdefault((p.device, group["state_bits"]), []).append(cohorts[key])
-                cohorts[key][2].append(p)
+                key = (device, id(step) if capturable else step)
+                cohort = cohorts.get(key)
+                if cohort is None:
+                    cohort = cohorts[key] = (group, step, [], [], [])
+                    launch = (device, group["state_bits"], group["seed"] if eight else 0)
+                    plan.setdefault(launch, []).append(cohort)
+                cohort[2].append(p)
+                cohort[3].append(grad)
+                cohort[4].append(st)
         return plan
 
     @torch.no_grad()
@@ -239,32 +245,30 @@ class AdamW(Optimizer):
             return loss
         scale = None
         if self.defaults["max_grad_norm"] > 0:
-            grads = [p.grad for parts in plan.values() for _, _, ps in parts for p in ps]
-            if len({g.device for g in grads}) > 1:
+            if len({device for device, _, _ in plan}) > 1:
                 raise ValueError("max_grad_norm needs every parameter on one device")
+            grads = [g for parts in plan.values() for part in parts for g in part[3]]
             self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
         ext = _ext.load()
-        for (_, bits), parts in plan.items():
+        for (_, bits, seed), parts in plan.items():
             for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
                 some = parts[at:at + _ADAMW_MAX_GROUPS]
                 groups = [(len(ps), g["lr"], g["betas"][0], g["betas"][1], g["eps"],
                            g["weight_decay"], step if g["capturable"] else step + 1)
-                          for g, step, ps in some]
-                params = [p for _, _, ps in some for p in ps]
-                grads = [p.grad for p in params]
-                states = [self.state[p] for p in params]
+                          for g, step, ps, _, _ in some]
+                params, grads, states = ([x for part in some for x in part[k]] for k in (2, 3, 4))
+                m, v = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq"))
                 if bits == 8:
-                    ext.adamw8_step(params, grads, [s["exp_avg"] for s in states],
-                                    [s["exp_avg_scales"] for s in states],
-                                    [s["exp_avg_sq"] for s in states],
-                                    [s["exp_avg_sq_scales"] for s in states], groups,
-                                    some[0][0]["seed"] & 0xFFFFFFFF, scale)
+                    ms, vs = ([s[k] for s in states]
+                              for k in ("exp_avg_scales", "exp_avg_sq_scales"))
+                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed & 0xFFFFFFFF,
+                                    scale)
                 else:
-                    ext.adamw_step(params, grads, [s["exp_avg"] for s in states],
-                                   [s["exp_avg_sq"] for s in states], groups, scale)
-                for s in states:
-                    if not isinstance(s["step"], torch.Tensor):
-                        s["step"] += 1
+                    ext.adamw_step(params, grads, m, v, groups, scale)
+                for g, step, _, _, sts in some:
+                    if not g["capturable"]:
+                        for st in sts:
+                            st["step"] = step + 1
         return loss
 
     @torch.no_grad()

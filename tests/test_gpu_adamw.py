@@ -769,6 +769,35 @@ def test_state_dict_round_trip(bits, capturable):
             other.step()
 
 
+def test_many_groups_of_every_kind_in_one_optimiser():
+    """More groups than a launch takes, 32- and 8-bit ones, own seeds, betas and
+    rates: the same as an optimiser for each group (8-bit: whose places in a list
+    are then others, so only one group of that kind for each seed)."""
+    def build():
+        gen = torch.Generator().manual_seed(2)
+        return [make(200 + 13 * i, [F32, BF16, F16][i % 3], gen, 0.3).requires_grad_()
+                for i in range(40)], gen
+
+    def options(i):
+        o = dict(lr=1e-3 * (i + 1), betas=(0.5 + 0.01 * i, 0.9), eps=1e-8 * (i + 1),
+                 weight_decay=0.01 * i)
+        return {**o, "state_bits": 8, "seed": i} if i % 10 == 7 else o
+    together, gen = build()
+    apart, _ = build()
+    opt = manbo.AdamW([{"params": [p], **options(i)} for i, p in enumerate(together)])
+    each = [manbo.AdamW([p], **options(i)) for i, p in enumerate(apart)]
+    for _ in range(3):
+        for p, q in zip(together, apart):
+            p.grad = make(p.numel(), p.dtype, gen)
+            q.grad = p.grad.clone()
+        opt.step()
+        for o in each:
+            o.step()
+    for p, q, o in zip(together, apart, each):
+        assert torch.equal(p, q)
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(p), o.moments(q)))
+
+
 def test_state_of_torch_adamw_loads_and_continues():
     """Two steps of torch's AdamW, then one here from its state, against float64
     from that state; what this class does not compute is refused."""
