@@ -62,11 +62,14 @@ struct AdamEntry8 {
   uint32_t block0;  // number of its first block in its tensor
 };
 
-// Bits 0-1 type, 2 vector path, 3-7 group, 8-31 place in the call's array.
-constexpr uint32_t entry_word(int dtype, bool vec, int group, int place) {
-  return (uint32_t)dtype | (vec ? 4u : 0u) | ((uint32_t)group << 3) | ((uint32_t)place << 8);
+// Bits 0-1 type, 2 everything aligned, 3-6 group, 7 moments aligned, 8-31 place
+// in the call's array.
+constexpr uint32_t kAligned = 4, kMomentsAligned = 128;
+constexpr uint32_t entry_word(int dtype, bool all, bool moments, int group, int place) {
+  return (uint32_t)dtype | (all ? kAligned : 0u) | ((uint32_t)group << 3) |
+         (moments ? kMomentsAligned : 0u) | ((uint32_t)place << 8);
 }
-static_assert(CS_ADAMW_MAX_GROUPS <= 32, "five bits of group");
+static_assert(CS_ADAMW_MAX_GROUPS <= 16, "four bits of group");
 
 template <class Entry, int N>
 struct Table {
@@ -149,6 +152,22 @@ __device__ __forceinline__ void store_wide(float* p, const float2 (&x)[4]) {
                : "memory");
 }
 
+// Two elements of a word or two, as float32.
+template <class T>
+__device__ __forceinline__ float2 unpack2(const uint32_t* w);
+template <>
+__device__ __forceinline__ float2 unpack2<float>(const uint32_t* w) {
+  return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(const uint32_t* w) {
+  return make_float2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(const uint32_t* w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(w));
+}
+
 struct StepCoef {
   float b1, omb1, b2, omb2, eps, step_size, decay, rbc2, scale;
   uint32_t key;
@@ -199,7 +218,7 @@ __device__ __forceinline__ void step_chunk(const AdamEntry& e, const StepCoef& c
   const int64_t left = e.numel - at - base;
   if (left <= 0) return;
   float P[8], G[8], M[8], V[8];
-  if ((e.word & 4) && left >= kBlock8) {
+  if ((e.word & kAligned) && left >= kBlock8) {
     const int i = base + lane * 8;
     load8(p + i, P);
     load8(g + i, G);
@@ -211,6 +230,8 @@ __device__ __forceinline__ void step_chunk(const AdamEntry& e, const StepCoef& c
     store8(m + i, M);
     store8(v + i, V);
   } else {
+    // by single elements 64 M float32 elements take as long as aligned ones (275
+    // us), bfloat16 ones 256 us (216)
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int i = base + lane + 32 * u;
@@ -239,7 +260,7 @@ __global__ void __launch_bounds__(kChunkThreads)
     adamw_kernel(const __grid_constant__ Table<AdamEntry, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 31], t.grad_scale);
+  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 15], t.grad_scale);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
   switch (e.word & 3) {
     case CS_F32: step_chunk<float>(e, c, at); break;
@@ -458,22 +479,6 @@ __device__ __forceinline__ void step_lane8(const StepCoef8& c, float2 (&P)[4],
   }
 }
 
-// Two elements of a word or two, as float32.
-template <class T>
-__device__ __forceinline__ float2 unpack2(const uint32_t* w);
-template <>
-__device__ __forceinline__ float2 unpack2<float>(const uint32_t* w) {
-  return bits2(w[0], w[1]);
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(const uint32_t* w) {
-  return bits2(w[0] << 16, w[0] & 0xFFFF0000u);
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(const uint32_t* w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(w));
-}
-
 // One lane's share of an aligned, full block as it lies in memory, and where.
 template <class T>
 struct Raw8 {
@@ -568,6 +573,70 @@ __device__ __forceinline__ void step_part8(const AdamEntry8& e, const StepCoef8&
   }
 }
 
+// A warp's 256 elements of an unaligned tensor, moved between memory (every 32nd
+// element a lane, so that an access is one stretch) and eight consecutive
+// elements a lane by way of the warp's kilobyte of shared memory.
+constexpr int kExchange = 64;  // uint4 a warp
+template <class T>
+__device__ __forceinline__ void load8_loose(const T* p, uint4* buf, int lane, float2 (&x)[4]) {
+  T* b = reinterpret_cast<T*>(buf);
+  T q[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) q[u] = p[lane + 32 * u];
+  __syncwarp();  // the last use of the buffer
+#pragma unroll
+  for (int u = 0; u < 8; ++u) b[lane + 32 * u] = q[u];
+  __syncwarp();
+  uint32_t w[2 * sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    const uint4 r = buf[lane * (sizeof(T) / 2) + i];
+    w[4 * i] = r.x;
+    w[4 * i + 1] = r.y;
+    w[4 * i + 2] = r.z;
+    w[4 * i + 3] = r.w;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) x[u] = unpack2<T>(w + u * (sizeof(T) / 2));
+}
+template <class T>
+__device__ __forceinline__ void store8_loose(T* p, uint4* buf, int lane, const float2 (&x)[4]) {
+  T* b = reinterpret_cast<T*>(buf);
+  __syncwarp();
+  store8(b + lane * 8, x);
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 8; ++u) p[lane + 32 * u] = b[lane + 32 * u];
+}
+
+// A full block whose codes are aligned and whose parameters or gradients are not:
+// 64 M float32 elements take 195 us, 300 by single elements throughout, 165
+// aligned; bfloat16 ones 245, 276 and 119 (their 16-bit accesses are what is
+// left).
+template <class T>
+__device__ __forceinline__ void step_loose8(const AdamEntry8& e, const StepCoef8& c,
+                                            uint32_t block, int lane, uint4* buf) {
+  const int64_t at = (int64_t)block * kBlock8;
+  T* p = static_cast<T*>(e.p) + at;
+  uint2* mc = reinterpret_cast<uint2*>(e.m + at) + lane;
+  uint2* vc = reinterpret_cast<uint2*>(e.v + at) + lane;
+  const uint2 a = *mc, b = *vc;
+  const uint32_t em = e.ms[block], ev = e.vs[block];
+  float2 P[4], G[4];
+  load8_loose(p, buf, lane, P);
+  load8_loose(static_cast<const T*>(e.g) + at, buf, lane, G);
+  uint32_t mw[2] = {a.x, a.y}, vw[2] = {b.x, b.y}, me, ve;
+  step_lane8<1>(c, P, G, mw, vw, c.b1 * scale_unit(em), c.b2 * scale_unit(ev),
+                block_key(c.key, e.word >> 8, e.block0 + block), lane * 8, me, ve);
+  store8_loose(p, buf, lane, P);
+  *mc = make_uint2(mw[0], mw[1]);
+  *vc = make_uint2(vw[0], vw[1]);
+  if (lane == 0) {
+    e.ms[block] = (uint8_t)me;
+    e.vs[block] = (uint8_t)ve;
+  }
+}
+
 // A warp's blocks: one of each kChunk that its CTA takes, which lie as far
 // apart as the tensor has CTAs, so that all CTAs together walk through memory
 // (neighbouring chunks for each CTA were 2.4 times slower: everything in flight
@@ -580,7 +649,7 @@ __device__ __forceinline__ void step_part8(const AdamEntry8& e, const StepCoef8&
 // SM, 698 us for 268 M elements instead of 643, and gain nothing at five).
 template <class T>
 __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8& c, uint32_t chunk,
-                                           int shift) {
+                                           int shift, uint4* buf) {
   constexpr uint32_t kWarps = kChunkThreads / 32;
   const int lane = threadIdx.x & 31;
   const uint32_t chunks = (uint32_t)((e.numel + kChunk - 1) / kChunk);
@@ -588,7 +657,8 @@ __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8&
   static_assert(kWarps == 4, "2 bits");
   const uint32_t first = chunk * kWarps + (threadIdx.x >> 5);
   const uint32_t end = (uint32_t)((e.numel + kBlock8 - 1) / kBlock8);
-  const uint32_t full = (e.word & 4) ? (uint32_t)(e.numel / kBlock8) : 0;
+  const uint32_t whole = (uint32_t)(e.numel / kBlock8);
+  const uint32_t full = (e.word & kAligned) ? whole : 0;
   int n = 0;  // full blocks of this warp
   if (first < full) n = shift ? (int)min(1u << shift, (full - first + stride - 1) / stride) : 1;
   if (n > 0) {
@@ -635,21 +705,27 @@ __device__ __forceinline__ void step_warp8(const AdamEntry8& e, const StepCoef8&
     }
   }
   for (uint32_t block = first + n * stride, i = n; i >> shift == 0 && block < end;
-       ++i, block += stride)
-    step_part8<T>(e, c, block, lane);
+       ++i, block += stride) {
+    if ((e.word & kMomentsAligned) && block < whole)
+      step_loose8<T>(e, c, block, lane, buf);
+    else
+      step_part8<T>(e, c, block, lane);
+  }
 }
 
 template <int N>
 __global__ void __launch_bounds__(kChunkThreads, 7)
     adamw8_kernel(const __grid_constant__ Table<AdamEntry8, N> t) {
+  __shared__ uint4 exchange[kChunkThreads / 32][kExchange];
+  uint4* buf = exchange[threadIdx.x >> 5];
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
-  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 31], t.grad_scale, t.one);
+  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 15], t.grad_scale, t.one);
   const int chunk = (int)blockIdx.x - t.first[k];
   switch (e.word & 3) {
-    case CS_F32: step_warp8<float>(e, c, chunk, t.shift); break;
-    case CS_BF16: step_warp8<__nv_bfloat16>(e, c, chunk, t.shift); break;
-    default: step_warp8<__half>(e, c, chunk, t.shift); break;
+    case CS_F32: step_warp8<float>(e, c, chunk, t.shift, buf); break;
+    case CS_BF16: step_warp8<__nv_bfloat16>(e, c, chunk, t.shift, buf); break;
+    default: step_warp8<__half>(e, c, chunk, t.shift, buf); break;
   }
 }
 
@@ -669,7 +745,7 @@ __global__ void __launch_bounds__(kChunkThreads)
   const uint8_t* mc = e.m + block * kBlock8;
   const uint8_t* vc = e.v + block * kBlock8;
   const float mb = scale_unit(e.ms[block]), vb = scale_unit(e.vs[block]);
-  if ((e.word & 4) && left >= kBlock8) {
+  if ((e.word & kAligned) && left >= kBlock8) {
     const uint2 a = *reinterpret_cast<const uint2*>(mc + lane * 8);
     const uint2 b = *reinterpret_cast<const uint2*>(vc + lane * 8);
     const float2 mk = pair(mb), vk = pair(vb), up112 = pair(kTwo112), up96 = pair(kTwo96);
@@ -1010,7 +1086,7 @@ struct GroupBuilder {
   }
 };
 
-// An entry holds elements [at, at + n) of a tensor.  The vector path needs
+// An entry holds elements [at, at + n) of a tensor.  Wide accesses need
 // parameters and gradients (in cs_adamw8_moments the outputs) aligned to
 // `width` bytes.
 inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
@@ -1024,9 +1100,9 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t a
   e.m = static_cast<float*>(s.exp_avg) + at;
   e.v = static_cast<float*>(s.exp_avg_sq) + at;
   e.numel = n;
-  const bool vec = aligned_to(e.p, width) && aligned_to(e.g, width) && aligned_to(e.m, 16) &&
-                   aligned_to(e.v, 16);
-  e.word = entry_word(s.dtype, vec, s.group, place);
+  const bool moments = aligned_to(e.m, 16) && aligned_to(e.v, 16);
+  e.word = entry_word(s.dtype, moments && aligned_to(e.p, width) && aligned_to(e.g, width),
+                      moments, s.group, place);
   e.pad = 0;
   return true;
 }
@@ -1044,9 +1120,9 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t a
   e.ms = s.exp_avg_scales + block;
   e.vs = s.exp_avg_sq_scales + block;
   e.numel = n;
-  const bool vec = aligned_to(e.p, width) && aligned_to(e.g, width) && aligned_to(e.m, 8) &&
-                   aligned_to(e.v, 8);
-  e.word = entry_word(s.dtype, vec, s.group, place);
+  const bool moments = aligned_to(e.m, 8) && aligned_to(e.v, 8);
+  e.word = entry_word(s.dtype, moments && aligned_to(e.p, width) && aligned_to(e.g, width),
+                      moments, s.group, place);
   e.block0 = (uint32_t)block;
   return true;
 }

@@ -387,6 +387,29 @@ def test_adamw8_step_of_views_leaves_their_surroundings(shift):
         assert torch.equal(x[:at], old[:at]) and torch.equal(x[at + k:], old[at + k:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shift", [1, 2, 7])
+@pytest.mark.parametrize("n", [255, 256, 1025, 5003])
+def test_unaligned_parameters_with_moments_of_their_own(n, shift, dtype):
+    """Views into a flat parameter buffer and a gradient bucket (only one of them
+    off its border, too), moments as an allocator gives them."""
+    gen = torch.Generator().manual_seed(n + shift)
+    flat, gflat = make(n + 16, dtype, gen, 0.3), make(n + 16, dtype, gen)
+    for at, gat in ((shift, shift), (0, shift), (shift, 8)):
+        p, g = flat[at:at + n], gflat[gat:gat + n]
+        old = flat.clone()
+        m, v = moments32(p, gen)
+        want = oa.adamw64(n64(p), n64(g), n64(m), n64(v), 7, **HYPER)
+        ops.adamw_step([p], [g], [m], [v], step=7, **HYPER)
+        check_param(p, dtype, want[0], want[3][0])
+        assert (np.abs(n64(m) - want[1]) <= want[3][1]).all()
+        assert (np.abs(n64(v) - want[2]) <= want[3][2]).all()
+        st = ops.adamw8_state(p)
+        for step in (1, 2):
+            step8_and_check([p], [g], [st], step, 0.7)
+        assert torch.equal(flat[:at], old[:at]) and torch.equal(flat[at + n:], old[at + n:])
+
+
 def test_adamw8_step_of_other_layouts():
     gen = torch.Generator().manual_seed(5)
     p = make(840, F32, gen).view(4, 6, 5, 7).contiguous(memory_format=torch.channels_last)
