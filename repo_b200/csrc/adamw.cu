@@ -1092,11 +1092,8 @@ struct GroupBuilder {
 // An entry holds elements [at, at + n) of a tensor.  Wide accesses need
 // parameters and gradients (in cs_adamw8_moments the outputs) aligned to
 // `width` bytes.
-inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
+inline void make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
                        AdamEntry& e) {
-  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !aligned_to(s.exp_avg, 4) ||
-      !aligned_to(s.exp_avg_sq, 4))
-    return false;
   const int64_t bytes = at * dtype_size(s.dtype);
   e.p = static_cast<char*>(s.param) + bytes;
   e.g = static_cast<const char*>(s.grad) + bytes;
@@ -1107,14 +1104,10 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t a
   e.word = entry_word(s.dtype, moments && aligned_to(e.p, width) && aligned_to(e.g, width),
                       moments, s.group, place);
   e.pad = 0;
-  return true;
 }
 
-inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
+inline void make_entry(const cs_adamw_tensor& s, int place, int width, int64_t at, int64_t n,
                        AdamEntry8& e) {
-  if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !s.exp_avg_scales ||
-      !s.exp_avg_sq_scales)
-    return false;
   const int64_t bytes = at * dtype_size(s.dtype), block = at / kBlock8;
   e.p = static_cast<char*>(s.param) + bytes;
   e.g = static_cast<const char*>(s.grad) + bytes;
@@ -1127,7 +1120,6 @@ inline bool make_entry(const cs_adamw_tensor& s, int place, int width, int64_t a
   e.word = entry_word(s.dtype, moments && aligned_to(e.p, width) && aligned_to(e.g, width),
                       moments, s.group, place);
   e.block0 = (uint32_t)block;
-  return true;
 }
 
 // A CTA takes several chunks (a power of two) where enough CTAs are left an SM:
@@ -1142,21 +1134,21 @@ constexpr int64_t ctas_wanted(int shift, bool half) {
 
 // The kernels of one table type, by name.
 struct RunStep {
-  static constexpr int kWidth = 16, kMostPer = 1;
+  static constexpr int kWidth = 16, kMostPer = 1, kMomentBytes = 4;
   template <int N>
   static void launch(const Table<AdamEntry, N>& t, int chunks, cudaStream_t st) {
     adamw_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunStep8 {
-  static constexpr int kWidth = 16, kMostPer = 32;
+  static constexpr int kWidth = 16, kMostPer = 32, kMomentBytes = 1;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
   }
 };
 struct RunMoments8 {
-  static constexpr int kWidth = 32, kMostPer = 1;
+  static constexpr int kWidth = 32, kMostPer = 1, kMomentBytes = 1;
   template <int N>
   static void launch(const Table<AdamEntry8, N>& t, int chunks, cudaStream_t st) {
     adamw8_moments_kernel<N><<<chunks, kChunkThreads, 0, st>>>(t);
@@ -1198,7 +1190,7 @@ int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const A
         t.count = 0;
         chunks = 0;
       }
-      if (!make_entry(s, i, Run::kWidth, at, n, t.e[t.count])) return CS_ERR_ARG;
+      make_entry(s, i, Run::kWidth, at, n, t.e[t.count]);
       t.first[t.count++] = (int)chunks;
       chunks += mine;
     }
@@ -1208,7 +1200,9 @@ int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const A
   return launch_status();
 }
 
-inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups) {
+// Everything that a call can refuse, before its first launch: `bytes` are those of
+// a moment's element, one with scales beside it.
+inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups, int bytes) {
   if (count < 0 || count > kMaxTensors || (count > 0 && !tensors)) return CS_ERR_ARG;
   for (int i = 0; i < count; ++i) {
     const cs_adamw_tensor& s = tensors[i];
@@ -1217,6 +1211,11 @@ inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups) 
       return CS_ERR_ARG;
     const int size = dtype_size(s.dtype);
     if (!aligned_to(s.param, size) || !aligned_to(s.grad, size)) return CS_ERR_ARG;
+    if (s.numel == 0) continue;
+    if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || !aligned_to(s.exp_avg, bytes) ||
+        !aligned_to(s.exp_avg_sq, bytes) ||
+        (bytes == 1 && (!s.exp_avg_scales || !s.exp_avg_sq_scales)))
+      return CS_ERR_ARG;
   }
   return CS_OK;
 }
@@ -1236,7 +1235,7 @@ int step_entry(const cs_adamw_tensor* tensors, int count, const cs_adamw_group* 
                int num_groups, const float* coef, uint32_t seed, const float* grad_scale,
                void* stream) {
   if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups) return CS_ERR_ARG;
-  if (int rc = check_tensors(tensors, count, num_groups)) return rc;
+  if (int rc = check_tensors(tensors, count, num_groups, Run::kMomentBytes)) return rc;
   GroupBuilder b;
   if (int rc = b.fill(groups, num_groups, coef, seed)) return rc;
   return run_tables<Run, Entry, kSmall, kLarge>(tensors, count, num_groups, b.g, grad_scale,
@@ -1338,7 +1337,7 @@ int cs_adamw8_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw
 }
 
 int cs_adamw8_moments(const cs_adamw_tensor* tensors, int32_t count, void* stream) {
-  if (int rc = check_tensors(tensors, count, 1)) return rc;
+  if (int rc = check_tensors(tensors, count, 1, RunMoments8::kMomentBytes)) return rc;
   for (int i = 0; i < count; ++i)
     if (tensors[i].dtype != CS_F32) return CS_ERR_ARG;
   return run_tables<RunMoments8, AdamEntry8, 36, 420>(tensors, count, 1, nullptr, nullptr,

@@ -1,0 +1,31 @@
+"""C calls whose tensors take more than one launch are refused as a whole, before
+the first one (no GPU needed: host addresses that no launch may see)."""
+import ctypes
+
+import pytest
+
+from repo_b200 import _native as nat
+from test_adamw_refusals import CS_ERR_ARG, CTensor, _group, _tensor
+
+BAD = (dict(exp_avg=None), dict(exp_avg_sq=None), dict(param=None), dict(grad=None))
+
+
+def _call(name, tensors):
+    t = (CTensor * len(tensors))(*tensors)
+    g = (type(_group()) * 1)(_group())
+    args = [ctypes.addressof(t), len(tensors)]
+    if name != "cs_adamw8_moments":
+        args += [ctypes.addressof(g), 1, None]
+    if name == "cs_adamw8_step":
+        args.append(7)
+    if name != "cs_adamw8_moments":
+        args.append(None)
+    return nat.call(name, *args, None)
+
+
+@pytest.mark.parametrize("name,bad", [
+    *(("cs_adamw_step", b) for b in (*BAD, dict(exp_avg=1026), dict(exp_avg_sq=2049))),
+    *((n, b) for n in ("cs_adamw8_step", "cs_adamw8_moments")
+      for b in (*BAD, dict(exp_avg_scales=None), dict(exp_avg_sq_scales=None)))])
+def test_a_bad_tensor_behind_a_full_table_is_refused_before_any_launch(name, bad):
+    assert _call(name, [_tensor()] * 1300 + [_tensor(**bad)]) == CS_ERR_ARG
