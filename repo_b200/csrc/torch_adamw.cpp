@@ -187,13 +187,21 @@ struct Written {
   }
 };
 
-// A 0-d (or one-element) float32 device scalar, or NULL for None.
+// The memory of one value of type T on `dev` (`want` says what it has to be).
+template <class T>
+T* device_value(const Tensor& t, const at::Device& dev, const std::string& name,
+                const char* want) {
+  if (t.layout() != at::kStrided || !t.is_cuda() || t.device() != dev ||
+      t.scalar_type() != c10::CppTypeToScalarType<T>::value || t.numel() != 1)
+    bad(name + " must be " + want + " on " + dev.str());
+  if (t.is_neg()) bad(name + " must not be a lazily negated view");
+  return t.data_ptr<T>();
+}
+
+// A float32 device scalar, or NULL for None.
 const float* device_scalar(const std::optional<Tensor>& t, const at::Device& dev,
                            const char* name) {
-  if (!t) return nullptr;
-  if (!t->is_cuda() || t->device() != dev || t->scalar_type() != at::kFloat || t->numel() != 1)
-    bad(std::string(name) + " must be one float32 value on " + dev.str());
-  return static_cast<const float*>(t->data_ptr());
+  return t ? device_value<float>(*t, dev, name, "one float32 value") : nullptr;
 }
 
 void* stream_of(const at::Device& dev) {
@@ -240,10 +248,8 @@ Groups read_groups(const py::list& list, Py_ssize_t tensors, const at::Device& d
       bad("Invalid weight_decay value: " + std::to_string(g.weight_decay));
     const py::handle step = t[6];
     if (is_scalar_tensor(step)) {
-      const Tensor& s = THPVariable_Unpack(step.ptr());
-      if (!s.is_cuda() || s.device() != dev || s.scalar_type() != at::kLong || s.numel() != 1)
-        bad("step must be an int or one int64 value on " + dev.str());
-      r.counters.push_back(s.data_ptr<int64_t>());
+      r.counters.push_back(device_value<int64_t>(THPVariable_Unpack(step.ptr()), dev, "step",
+                                                 "an int or one int64 value"));
     } else {
       g.step = step.cast<int64_t>();
       if (g.step < 1) bad("step must be >= 1, got " + std::to_string(g.step));

@@ -49,3 +49,18 @@ def test_a_learning_rate_of_zero_with_a_square_that_overflows():
         m, v = torch.zeros(600, device="cuda"), torch.zeros(600, device="cuda")
         ops.adamw_step([p], [g], [m], [v], step=1, lr=0.0)
         assert torch.equal(p, old)
+
+
+def test_lazily_negated_scalars_are_refused():
+    p, g, m, v = (torch.ones(8, device="cuda") for _ in range(4))
+    neg = torch._neg_view(torch.full((), 0.5, device="cuda"))
+    st = ops.adamw8_state(p)
+    for kw, name in ((dict(lr=neg), "lr"), (dict(grad_scale=neg), "grad_scale")):
+        with pytest.raises(ValueError, match=f"{name} must not be a lazily negated"):
+            ops.adamw_step([p], [g], [m], [v], step=1, **kw)
+        with pytest.raises(ValueError, match=f"{name} must not be a lazily negated"):
+            ops.adamw8_step([p], [g], *[[x] for x in st], step=1, **kw)
+    count = torch._neg_view(torch.full((), 5, device="cuda"))
+    with pytest.raises(ValueError, match="step must not be a lazily negated"):
+        ops.adamw_step([p], [g], [m], [v], step=count)
+    assert torch.equal(p, torch.ones_like(p))
