@@ -214,6 +214,7 @@ struct Groups {
   std::vector<cs_adamw_group> g;
   std::vector<int64_t> ends;     // one past each group's last tensor
   std::vector<int64_t*> counters;  // device step counters, or empty
+  std::vector<Impl*> changed;      // their tensors
 };
 
 // groups: (tensors, lr, beta1, beta2, eps, weight_decay, step) each; lr a float
@@ -248,8 +249,9 @@ Groups read_groups(const py::list& list, Py_ssize_t tensors, const at::Device& d
       bad("Invalid weight_decay value: " + std::to_string(g.weight_decay));
     const py::handle step = t[6];
     if (is_scalar_tensor(step)) {
-      r.counters.push_back(device_value<int64_t>(THPVariable_Unpack(step.ptr()), dev, "step",
-                                                 "an int or one int64 value"));
+      const Tensor& s = THPVariable_Unpack(step.ptr());
+      r.counters.push_back(device_value<int64_t>(s, dev, "step", "an int or one int64 value"));
+      r.changed.push_back(s.unsafeGetTensorImpl());
     } else {
       g.step = step.cast<int64_t>();
       if (g.step < 1) bad("step must be >= 1, got " + std::to_string(g.step));
@@ -333,8 +335,8 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
-  std::vector<Impl*> changed;
-  changed.reserve(params.n);
+  std::vector<Impl*> changed = r.changed;
+  changed.reserve(changed.size() + 3 * params.n);
   Written written(3 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
@@ -345,6 +347,8 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     check_like(mi, p, contiguous, m, i);
     check_like(vi, p, contiguous, v, i);
     if (!s.numel) continue;
+    changed.push_back(mi);
+    changed.push_back(vi);
     written.add(s.exp_avg = m.data(mi), m, i);
     written.add(s.exp_avg_sq = v.data(vi), v, i);
   }
@@ -374,8 +378,8 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
   const float* scale = device_scalar(grad_scale, dev, "grad_scale");
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
-  std::vector<Impl*> changed;
-  changed.reserve(params.n);
+  std::vector<Impl*> changed = r.changed;
+  changed.reserve(changed.size() + 5 * params.n);
   Written written(5 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
@@ -390,6 +394,7 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
     check_scales(msi, scale_count(s.numel), ms, i);
     check_scales(vsi, scale_count(s.numel), vs, i);
     if (!s.numel) continue;
+    for (Impl* x : {mi, vi, msi, vsi}) changed.push_back(x);
     written.add(s.exp_avg = m.data(mi), m, i);
     written.add(s.exp_avg_sq = v.data(vi), v, i);
     written.add(s.exp_avg_scales = static_cast<uint8_t*>(ms.data(msi)), ms, i);

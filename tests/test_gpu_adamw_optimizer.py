@@ -64,3 +64,24 @@ def test_lazily_negated_scalars_are_refused():
     with pytest.raises(ValueError, match="step must not be a lazily negated"):
         ops.adamw_step([p], [g], [m], [v], step=count)
     assert torch.equal(p, torch.ones_like(p))
+
+
+def test_written_moments_and_counters_rise_in_version():
+    p, g = torch.ones(600, device="cuda"), torch.ones(600, device="cuda")
+    m, v = torch.zeros(600, device="cuda"), torch.zeros(600, device="cuda")
+    count = torch.zeros((), dtype=torch.int64, device="cuda")
+    x = torch.ones(600, device="cuda", requires_grad=True)
+    y = (x * m).sum()
+    ops.adamw_step([p], [g], [m], [v], step=count)
+    assert all(t._version == 1 for t in (p, m, v, count)) and g._version == 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    st = ops.adamw8_state(p)
+    before = [t._version for t in st]
+    ops.adamw8_step([p], [g], *[[t] for t in st], step=count)
+    assert [t._version for t in st] == [b + 1 for b in before]
+    assert p._version == 2 and count._version == 2 and g._version == 0
+    out = [torch.zeros(600, device="cuda")], [torch.zeros(600, device="cuda")]
+    ops.adamw8_moments(*[[t] for t in st], out=out)
+    assert out[0][0]._version == 1 and out[1][0]._version == 1
+    assert [t._version for t in st] == [b + 1 for b in before]
