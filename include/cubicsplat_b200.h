@@ -425,11 +425,17 @@ CS_API int cs_adamw_step(const cs_adamw_tensor *tensors, int32_t count,
  * each block of 256: m is a sign, 4 exponent and 3 fraction bits, v 5 exponent
  * and 3 fraction bits, both with gradual underflow, in units of 2^(E-127);
  * E = 255 marks a block that is not finite.  Zeroed bytes stand for zero.  An eps
- * below 2^-60, the root of the smallest v, counts as 2^-60.  The bytes are rounded stochastically from a hash of (seed, t, place of the tensor
- * in the array, element), so a call is reproducible. */
+ * below 2^-60, the root of the smallest v, counts as 2^-60.  The bytes are rounded
+ * stochastically from a hash of (seed, t, place of the tensor in the array, element),
+ * so a call is reproducible. */
 CS_API int cs_adamw8_step(const cs_adamw_tensor *tensors, int32_t count,
                    const cs_adamw_group *groups, int32_t num_groups, const float *coef,
                    uint32_t seed, const float *grad_scale, void *stream);
+/* The same for tensors of a longer list: the first one's place is first_place, so
+ * that a list which takes several calls draws no random bits twice. */
+CS_API int cs_adamw8_step_at(const cs_adamw_tensor *tensors, int32_t count,
+                      const cs_adamw_group *groups, int32_t num_groups, const float *coef,
+                      uint32_t seed, int32_t first_place, const float *grad_scale, void *stream);
 
 /* Values of 8-bit moments: param and grad point to the float outputs for m and
  * v (both written), dtype is CS_F32, group 0. */

@@ -250,6 +250,7 @@ class AdamW(Optimizer):
             grads = [g for parts in plan.values() for part in parts for g in part[3]]
             self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
         ext = _ext.load()
+        places = {}  # 8-bit parameters already stepped with a seed, which draw other bits
         for (_, bits, seed), parts in plan.items():
             for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
                 some = parts[at:at + _ADAMW_MAX_GROUPS]
@@ -261,8 +262,10 @@ class AdamW(Optimizer):
                 if bits == 8:
                     ms, vs = ([s[k] for s in states]
                               for k in ("exp_avg_scales", "exp_avg_sq_scales"))
-                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed & 0xFFFFFFFF,
-                                    scale)
+                    seed &= 0xFFFFFFFF
+                    first = places.get(seed, 0)
+                    places[seed] = first + len(params)
+                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed, scale, first)
                 else:
                     ext.adamw_step(params, grads, m, v, groups, scale)
                 for g, step, _, _, sts in some:

@@ -76,6 +76,7 @@ struct Table {
   int count;
   int shift;  // a CTA takes 2^shift kChunks
   float one;  // 1 (see sum2)
+  uint32_t place_key;  // of the place that the call's first tensor has
   const float* grad_scale;
   AdamGroup groups[CS_ADAMW_MAX_GROUPS];
   int first[N];  // first chunk of each entry
@@ -305,8 +306,9 @@ __host__ __device__ constexpr uint32_t mix32(uint32_t h) {
 __host__ __device__ constexpr uint32_t step_key(uint32_t seed, uint32_t step) {
   return mix32(seed + step * 0x9E3779B1u);
 }
+__host__ __device__ constexpr uint32_t place_key(uint32_t place) { return place * 0x3C6EF373u; }
 __device__ __forceinline__ uint32_t block_key(uint32_t key, uint32_t place, uint32_t block) {
-  return mix32(key + place * 0x3C6EF373u + block * 0xA54FF53Bu);
+  return mix32(key + place_key(place) + block * 0xA54FF53Bu);
 }
 __device__ __forceinline__ float scale_unit(uint32_t e) {
   const float x = __uint_as_float(e << 23);  // infinity for 255
@@ -379,7 +381,7 @@ struct StepCoef8 {
 // near or at zero makes off infinite, which moves nothing; root stays finite, so
 // that neither its product with v = 0 nor an infinite v with it is NaN.
 __device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float* grad_scale,
-                                                float one) {
+                                                float one, uint32_t place_key) {
   const StepCoef s = load_coef(g, grad_scale);
   StepCoef8 c;
   c.b1 = s.b1;
@@ -391,7 +393,7 @@ __device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float*
   c.decay = s.decay;
   c.root = fminf(fmaxf(__fdividef(-s.rbc2, s.step_size), -kLargest), kLargest);
   c.off = __fdividef(-fmaxf(s.eps, kLeastEps), s.step_size);
-  c.key = s.key;
+  c.key = s.key + place_key;
   return c;
 }
 
@@ -723,7 +725,7 @@ __global__ void __launch_bounds__(kChunkThreads, 7)
   uint4* buf = exchange[threadIdx.x >> 5];
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
-  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 15], t.grad_scale, t.one);
+  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 15], t.grad_scale, t.one, t.place_key);
   const int chunk = (int)blockIdx.x - t.first[k];
   switch (e.word & 3) {
     case CS_F32: step_warp8<float>(e, c, chunk, t.shift, buf); break;
@@ -1158,10 +1160,11 @@ struct RunMoments8 {
 // Packs tensors (empty ones left out) into tables of at most N entries and
 // launches each full one.
 template <class Run, class Entry, int N>
-int launch_tables(const cs_adamw_tensor* tensors, int count, int groups, const AdamGroup* g,
+int launch_tables(const cs_adamw_tensor* tensors, int count, int first_place, const AdamGroup* g,
                   const float* grad_scale, cudaStream_t st) {
   Table<Entry, N> t;
   t.one = 1.0f;
+  t.place_key = place_key((uint32_t)first_place);
   t.grad_scale = grad_scale;
   for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
   int64_t total = 0;
@@ -1222,23 +1225,24 @@ inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups, 
 
 // A call of few tensors takes a small table (its parameters stay below 4 KB).
 template <class Run, class Entry, int kSmall, int kLarge>
-int run_tables(const cs_adamw_tensor* tensors, int count, int groups, const AdamGroup* g,
+int run_tables(const cs_adamw_tensor* tensors, int count, int first_place, const AdamGroup* g,
                const float* grad_scale, cudaStream_t st) {
   static_assert(sizeof(Table<Entry, kLarge>) <= 32764, "kernel parameter limit");
   if (count <= kSmall)
-    return launch_tables<Run, Entry, kSmall>(tensors, count, groups, g, grad_scale, st);
-  return launch_tables<Run, Entry, kLarge>(tensors, count, groups, g, grad_scale, st);
+    return launch_tables<Run, Entry, kSmall>(tensors, count, first_place, g, grad_scale, st);
+  return launch_tables<Run, Entry, kLarge>(tensors, count, first_place, g, grad_scale, st);
 }
 
 template <class Run, class Entry, int kSmall, int kLarge>
 int step_entry(const cs_adamw_tensor* tensors, int count, const cs_adamw_group* groups,
-               int num_groups, const float* coef, uint32_t seed, const float* grad_scale,
-               void* stream) {
-  if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups) return CS_ERR_ARG;
+               int num_groups, const float* coef, uint32_t seed, int first_place,
+               const float* grad_scale, void* stream) {
+  if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups || first_place < 0)
+    return CS_ERR_ARG;
   if (int rc = check_tensors(tensors, count, num_groups, Run::kMomentBytes)) return rc;
   GroupBuilder b;
   if (int rc = b.fill(groups, num_groups, coef, seed)) return rc;
-  return run_tables<Run, Entry, kSmall, kLarge>(tensors, count, num_groups, b.g, grad_scale,
+  return run_tables<Run, Entry, kSmall, kLarge>(tensors, count, first_place, b.g, grad_scale,
                                                 (cudaStream_t)stream);
 }
 
@@ -1325,22 +1329,28 @@ extern "C" {
 
 int cs_adamw_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
                   int32_t num_groups, const float* coef, const float* grad_scale, void* stream) {
-  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, coef, 0,
+  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, coef, 0, 0,
                                                  grad_scale, stream);
+}
+
+int cs_adamw8_step_at(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
+                      int32_t num_groups, const float* coef, uint32_t seed, int32_t first_place,
+                      const float* grad_scale, void* stream) {
+  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, coef, seed,
+                                                   first_place, grad_scale, stream);
 }
 
 int cs_adamw8_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
                    int32_t num_groups, const float* coef, uint32_t seed, const float* grad_scale,
                    void* stream) {
-  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, coef, seed,
-                                                   grad_scale, stream);
+  return cs_adamw8_step_at(tensors, count, groups, num_groups, coef, seed, 0, grad_scale, stream);
 }
 
 int cs_adamw8_moments(const cs_adamw_tensor* tensors, int32_t count, void* stream) {
   if (int rc = check_tensors(tensors, count, 1, RunMoments8::kMomentBytes)) return rc;
   for (int i = 0; i < count; ++i)
     if (tensors[i].dtype != CS_F32) return CS_ERR_ARG;
-  return run_tables<RunMoments8, AdamEntry8, 36, 420>(tensors, count, 1, nullptr, nullptr,
+  return run_tables<RunMoments8, AdamEntry8, 36, 420>(tensors, count, 0, nullptr, nullptr,
                                                       (cudaStream_t)stream);
 }
 

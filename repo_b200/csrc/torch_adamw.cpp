@@ -364,7 +364,7 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
 void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
                  const py::object& m_scales_, const py::object& exp_avg_sqs_,
                  const py::object& v_scales_, const py::list& groups, uint32_t seed,
-                 const std::optional<Tensor>& grad_scale) {
+                 const std::optional<Tensor>& grad_scale, int32_t first_place) {
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       ms(m_scales_, "exp_avg_scales"), v(exp_avg_sqs_, "exp_avg_sqs"),
       vs(v_scales_, "exp_avg_sq_scales");
@@ -402,10 +402,10 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
   }
   set_groups(r, t);
   const std::optional<Tensor> coef = advance(r, seed, dev);
-  check(cs_adamw8_step(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                       coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed, scale,
-                       stream_of(dev)),
-        "cs_adamw8_step");
+  check(cs_adamw8_step_at(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
+                          coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed,
+                          first_place, scale, stream_of(dev)),
+        "cs_adamw8_step_at");
   bump_versions(changed);
 }
 

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from repo_b200 import _native as nat
-from test_adamw_refusals import CS_ERR_ARG, CTensor, _group, _tensor
+from test_adamw_refusals import CS_ERR_ARG, CS_OK, CTensor, _group, _tensor
 
 BAD = (dict(exp_avg=None), dict(exp_avg_sq=None), dict(param=None), dict(grad=None))
 
@@ -29,3 +29,11 @@ def _call(name, tensors):
       for b in (*BAD, dict(exp_avg_scales=None), dict(exp_avg_sq_scales=None)))])
 def test_a_bad_tensor_behind_a_full_table_is_refused_before_any_launch(name, bad):
     assert _call(name, [_tensor()] * 1300 + [_tensor(**bad)]) == CS_ERR_ARG
+
+
+def test_a_first_place_below_zero_is_refused():
+    t, g = (CTensor * 1)(_tensor()), (type(_group()) * 1)(_group())
+    for place, tensor, want in ((-1, _tensor(), CS_ERR_ARG), (5, _tensor(numel=0), CS_OK)):
+        t[0] = tensor
+        assert nat.call("cs_adamw8_step_at", ctypes.addressof(t), 1, ctypes.addressof(g), 1, None,
+                        7, place, None, None) == want

@@ -85,3 +85,24 @@ def test_written_moments_and_counters_rise_in_version():
     ops.adamw8_moments(*[[t] for t in st], out=out)
     assert out[0][0]._version == 1 and out[1][0]._version == 1
     assert [t._version for t in st] == [b + 1 for b in before]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_groups_beyond_one_launch_round_with_bits_of_their_own(capturable):
+    """40 groups of one seed: each parameter's codes are those of its place in the
+    whole step (of the restatement), not of its place in a launch."""
+    ps, gen = params_of([600] * 40, seed=7)
+    opt = manbo.AdamW([{"params": [p], "lr": 1e-3 * (i + 1)} for i, p in enumerate(ps)],
+                      state_bits=8, capturable=capturable, seed=11)
+    zeros, scales = np.zeros(600, np.uint8), np.zeros(3, np.uint8)
+    state = [(zeros, scales, zeros, scales)] * 40
+    for t in (1, 2):
+        for i, p in enumerate(ps):
+            p.grad = make(600, F32, gen)
+            state[i] = oa.step8(p.grad.cpu().numpy(), *state[i], step=t, seed=11, place=i)[2:]
+        opt.step()
+        for p, want in zip(ps, state):
+            st = opt.state[p]
+            for k, w in zip(("exp_avg", "exp_avg_scales", "exp_avg_sq", "exp_avg_sq_scales"),
+                            want):
+                np.testing.assert_array_equal(st[k].cpu().numpy(), w)
