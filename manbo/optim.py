@@ -199,8 +199,8 @@ class AdamW(Optimizer):
         return st
 
     def _plan(self):
-        """{(device index, state_bits, seed): [(group, step, parameters, gradients,
-        states)]} of this step, the parameters of an entry at the same step."""
+        """{(device index, state_bits, seed, capturable): [(group, step, parameters,
+        gradients, states)]} of this step, the parameters of an entry at the same step."""
         plan = {}
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for group in self.param_groups:
@@ -227,7 +227,8 @@ class AdamW(Optimizer):
                 cohort = cohorts.get(key)
                 if cohort is None:
                     cohort = cohorts[key] = (group, step, [], [], [])
-                    launch = (device, group["state_bits"], group["seed"] if eight else 0)
+                    launch = (device, group["state_bits"], group["seed"] if eight else 0,
+                              capturable)
                     plan.setdefault(launch, []).append(cohort)
                 cohort[2].append(p)
                 cohort[3].append(grad)
@@ -245,13 +246,13 @@ class AdamW(Optimizer):
             return loss
         scale = None
         if self.defaults["max_grad_norm"] > 0:
-            if len({device for device, _, _ in plan}) > 1:
+            if len({device for device, *_ in plan}) > 1:
                 raise ValueError("max_grad_norm needs every parameter on one device")
             grads = [g for parts in plan.values() for part in parts for g in part[3]]
             self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
         ext = _ext.load()
         places = {}  # 8-bit parameters already stepped with a seed, which draw other bits
-        for (_, bits, seed), parts in plan.items():
+        for (_, bits, seed, _), parts in plan.items():
             for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
                 some = parts[at:at + _ADAMW_MAX_GROUPS]
                 groups = [(len(ps), g["lr"], g["betas"][0], g["betas"][1], g["eps"],

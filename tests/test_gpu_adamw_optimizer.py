@@ -106,3 +106,18 @@ def test_groups_beyond_one_launch_round_with_bits_of_their_own(capturable):
             for k, w in zip(("exp_avg", "exp_avg_scales", "exp_avg_sq", "exp_avg_sq_scales"),
                             want):
                 np.testing.assert_array_equal(st[k].cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_groups_may_differ_in_capturable(bits):
+    runs = []
+    for mixed in (False, True):
+        ps, gen = params_of((300, 700, 50), seed=6)
+        opt = manbo.AdamW([{"params": [p], "capturable": mixed and i != 1, "seed": i}
+                           for i, p in enumerate(ps)], lr=0.01, state_bits=bits)
+        for _ in range(3):
+            for p in ps:
+                p.grad = make(p.numel(), F32, gen)
+            opt.step()
+        runs.append([x for p in ps for x in (p, *opt.moments(p))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
