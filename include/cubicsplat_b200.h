@@ -446,6 +446,19 @@ CS_API int cs_adamw8_moments(const cs_adamw_tensor *tensors, int32_t count, void
 CS_API int cs_adamw_advance(int64_t *const *steps, const cs_adamw_group *groups,
                      int32_t num_groups, uint32_t seed, float *coef, void *stream);
 
+/* The steps with a device counter for each tensor (steps[i], no two the same):
+ * every one is advanced, those of empty tensors too, and then numbers its tensor's
+ * step.  workspace: 16 bytes a tensor on the device, in any state, not shared with
+ * a call that may run at the same time. */
+CS_API int cs_adamw_step_counted(const cs_adamw_tensor *tensors, int32_t count,
+                          const cs_adamw_group *groups, int32_t num_groups,
+                          int64_t *const *steps, float *workspace, const float *grad_scale,
+                          void *stream);
+CS_API int cs_adamw8_step_counted(const cs_adamw_tensor *tensors, int32_t count,
+                           const cs_adamw_group *groups, int32_t num_groups,
+                           int64_t *const *steps, float *workspace, uint32_t seed,
+                           int32_t first_place, const float *grad_scale, void *stream);
+
 typedef struct cs_grad_tensor {
   const void *data;
   int64_t numel;

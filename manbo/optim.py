@@ -140,12 +140,10 @@ class AdamW(Optimizer):
     on the device (``grad_norm`` holds the last one).  Parameters are float32,
     bfloat16 or float16, non-overlapping and dense.
 
-    Steps are counted per parameter, from the first step at which it has a
-    gradient.  With ``capturable`` the count lives on the device, one counter for
-    the parameters of a group that get their first gradient in the same step, so
-    that a captured step counts on every replay; a group's ``lr`` may then be a
-    float32 device scalar that a schedule writes to.  Take one step before the
-    capture, so that the state exists.
+    Steps are counted per parameter, those at which it has a gradient.  With
+    ``capturable`` the counts live on the device, so that a captured step counts on
+    every replay; a group's ``lr`` may then be a float32 device scalar that a
+    schedule writes to.  Take one step before the capture, so that the state exists.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -179,7 +177,7 @@ class AdamW(Optimizer):
             for key, value in self.defaults.items():
                 group.setdefault(key, value)
 
-    def _new_state(self, p, group, counters, capturing):
+    def _new_state(self, p, group, capturing):
         if capturing:
             raise RuntimeError("AdamW: take one step before capturing, so that the state exists")
         st = {}
@@ -190,21 +188,18 @@ class AdamW(Optimizer):
             for k in ("exp_avg", "exp_avg_sq"):
                 st[k] = torch.zeros_like(p, dtype=torch.float32,
                                          memory_format=torch.preserve_format)
-        if group["capturable"]:
-            if p.device not in counters:
-                counters[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
-            st["step"] = counters[p.device]
-        else:
-            st["step"] = 0
+        st["step"] = (torch.zeros((), dtype=torch.int64, device=p.device) if group["capturable"]
+                      else 0)
         return st
 
     def _plan(self):
         """{(device index, state_bits, seed, capturable): [(group, step, parameters,
-        gradients, states)]} of this step, the parameters of an entry at the same step."""
+        gradients, states)]} of this step, the parameters of an entry at the same step
+        (counted on the device, step is None and they may be at any)."""
         plan = {}
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for group in self.param_groups:
-            cohorts, counters = {}, {}
+            cohorts = {}
             eight, capturable = group["state_bits"] == 8, bool(group["capturable"])
             if capturing and not capturable:
                 raise RuntimeError("AdamW: a captured step needs capturable=True")
@@ -217,13 +212,15 @@ class AdamW(Optimizer):
                     raise ValueError("AdamW parameters must be CUDA tensors")
                 st = self.state[p]
                 if not st:
-                    st.update(self._new_state(p, group, counters, capturing))
+                    st.update(self._new_state(p, group, capturing))
                 if ("exp_avg_scales" in st) != eight:
                     raise ValueError(f"AdamW state is not of state_bits={group['state_bits']}")
                 step = st["step"]
                 if isinstance(step, torch.Tensor) != capturable:
                     raise ValueError("AdamW state was made with another value of capturable")
-                key = (device, id(step) if capturable else step)
+                if capturable:
+                    step = None
+                key = (device, step)
                 cohort = cohorts.get(key)
                 if cohort is None:
                     cohort = cohorts[key] = (group, step, [], [], [])
@@ -252,25 +249,27 @@ class AdamW(Optimizer):
             self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
         ext = _ext.load()
         places = {}  # 8-bit parameters already stepped with a seed, which draw other bits
-        for (_, bits, seed, _), parts in plan.items():
+        for (_, bits, seed, capturable), parts in plan.items():
             for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
                 some = parts[at:at + _ADAMW_MAX_GROUPS]
                 groups = [(len(ps), g["lr"], g["betas"][0], g["betas"][1], g["eps"],
-                           g["weight_decay"], step if g["capturable"] else step + 1)
+                           g["weight_decay"], 1 if capturable else step + 1)
                           for g, step, ps, _, _ in some]
                 params, grads, states = ([x for part in some for x in part[k]] for k in (2, 3, 4))
                 m, v = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq"))
+                steps = [s["step"] for s in states] if capturable else None
                 if bits == 8:
                     ms, vs = ([s[k] for s in states]
                               for k in ("exp_avg_scales", "exp_avg_sq_scales"))
                     seed &= 0xFFFFFFFF
                     first = places.get(seed, 0)
                     places[seed] = first + len(params)
-                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed, scale, first)
+                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed, scale, first,
+                                    steps)
                 else:
-                    ext.adamw_step(params, grads, m, v, groups, scale)
-                for g, step, _, _, sts in some:
-                    if not g["capturable"]:
+                    ext.adamw_step(params, grads, m, v, groups, scale, steps)
+                if not capturable:
+                    for _, step, _, _, sts in some:
                         for st in sts:
                             st["step"] = step + 1
         return loss
@@ -304,7 +303,6 @@ class AdamW(Optimizer):
         super().load_state_dict({**state_dict, "state": {}})
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         own = [(p, g) for g in self.param_groups for p in g["params"]]
-        counters = {}
         for i, (p, group) in zip(ids, own):
             if i not in state_dict["state"]:
                 continue
@@ -315,14 +313,9 @@ class AdamW(Optimizer):
                                  "saved with (their blocks follow its storage)")
             for k, x in state_dict["state"][i].items():
                 if k == "step":
-                    if not group["capturable"]:
-                        st[k] = int(x)
-                    else:  # parameters that shared a counter share the new one
-                        key = (id(group), id(x) if isinstance(x, torch.Tensor) else x, p.device)
-                        if key not in counters:
-                            counters[key] = torch.tensor(int(x), dtype=torch.int64,
-                                                         device=p.device)
-                        st[k] = counters[key]
+                    st[k] = int(x)
+                    if group["capturable"]:
+                        st[k] = torch.tensor(st[k], dtype=torch.int64, device=p.device)
                 elif isinstance(x, torch.Tensor):
                     y = torch.empty_like(p, dtype=x.dtype) if x.shape == p.shape \
                         else torch.empty_like(x, device=p.device)

@@ -86,6 +86,9 @@ SIGNATURES = {
     "cs_adamw_step": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P]),
     "cs_adamw8_step": (ctypes.c_int, [_P, _I32, _P, _I32, _P, ctypes.c_uint32, _P, _P]),
     "cs_adamw8_step_at": (ctypes.c_int, [_P, _I32, _P, _I32, _P, ctypes.c_uint32, _I32, _P, _P]),
+    "cs_adamw_step_counted": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _P]),
+    "cs_adamw8_step_counted": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, ctypes.c_uint32, _I32,
+                                              _P, _P]),
     "cs_adamw8_moments": (ctypes.c_int, [_P, _I32, _P]),
     "cs_adamw_advance": (ctypes.c_int, [_P, _P, _I32, ctypes.c_uint32, _P, _P]),
     "cs_grad_norm_workspace_size": (_SZ, [_P, _I32]),

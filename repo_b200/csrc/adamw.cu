@@ -37,7 +37,6 @@ struct AdamGroup {
   float b1, omb1, b2, omb2, eps, lr, wd, ibc1, rbc2;  // ibc1 = 1/(1-b1^t), rbc2 = 1/sqrt(1-b2^t)
   uint32_t key;                                       // of the stochastic rounding
   const float* lr_dev;                                // replaces lr where given
-  const float* coef;                                  // {ibc1, rbc2, key bits} where given
 };
 
 struct AdamEntry {
@@ -78,6 +77,8 @@ struct Table {
   float one;  // 1 (see sum2)
   uint32_t place_key;  // of the place that the call's first tensor has
   const float* grad_scale;
+  const float* coef;  // {ibc1, rbc2, key bits, -} of each group, or of each tensor; or NULL
+  int each;           // of each tensor
   AdamGroup groups[CS_ADAMW_MAX_GROUPS];
   int first[N];  // first chunk of each entry
   Entry e[N];
@@ -174,7 +175,10 @@ struct StepCoef {
   uint32_t key;
 };
 
-__device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* grad_scale) {
+template <class Entry, int N>
+__device__ __forceinline__ StepCoef load_coef(const Table<Entry, N>& t, uint32_t word) {
+  const uint32_t group = (word >> 3) & 15;
+  const AdamGroup& g = t.groups[group];
   StepCoef c;
   c.b1 = g.b1;
   c.omb1 = g.omb1;
@@ -185,14 +189,15 @@ __device__ __forceinline__ StepCoef load_coef(const AdamGroup& g, const float* g
   float ibc1 = g.ibc1;
   c.rbc2 = g.rbc2;
   c.key = g.key;
-  if (g.coef) {
-    ibc1 = __ldg(g.coef);
-    c.rbc2 = __ldg(g.coef + 1);
-    c.key = __float_as_uint(__ldg(g.coef + 2));
+  if (t.coef) {
+    const float* coef = t.coef + 4 * (t.each ? word >> 8 : group);
+    ibc1 = __ldg(coef);
+    c.rbc2 = __ldg(coef + 1);
+    c.key = __float_as_uint(__ldg(coef + 2));
   }
   c.step_size = lr * ibc1;
   c.decay = __fmaf_rn(-lr, g.wd, 1.0f);
-  c.scale = grad_scale ? __ldg(grad_scale) : 1.0f;
+  c.scale = t.grad_scale ? __ldg(t.grad_scale) : 1.0f;
   return c;
 }
 
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(kChunkThreads)
     adamw_kernel(const __grid_constant__ Table<AdamEntry, N> t) {
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry& e = t.e[k];
-  const StepCoef c = load_coef(t.groups[(e.word >> 3) & 15], t.grad_scale);
+  const StepCoef c = load_coef(t, e.word);
   const int64_t at = (int64_t)((int)blockIdx.x - t.first[k]) * kChunk;
   switch (e.word & 3) {
     case CS_F32: step_chunk<float>(e, c, at); break;
@@ -380,20 +385,20 @@ struct StepCoef8 {
 // holds) and the correction of v, both over the negative step size.  A step size
 // near or at zero makes off infinite, which moves nothing; root stays finite, so
 // that neither its product with v = 0 nor an infinite v with it is NaN.
-__device__ __forceinline__ StepCoef8 load_coef8(const AdamGroup& g, const float* grad_scale,
-                                                float one, uint32_t place_key) {
-  const StepCoef s = load_coef(g, grad_scale);
+template <int N>
+__device__ __forceinline__ StepCoef8 load_coef8(const Table<AdamEntry8, N>& t, uint32_t word) {
+  const StepCoef s = load_coef(t, word);
   StepCoef8 c;
   c.b1 = s.b1;
   c.b2 = s.b2;
   c.omb1 = s.omb1;
   c.omb2 = s.omb2;
   c.scale = s.scale;
-  c.one = one;
+  c.one = t.one;
   c.decay = s.decay;
   c.root = fminf(fmaxf(__fdividef(-s.rbc2, s.step_size), -kLargest), kLargest);
   c.off = __fdividef(-fmaxf(s.eps, kLeastEps), s.step_size);
-  c.key = s.key + place_key;
+  c.key = s.key + t.place_key;
   return c;
 }
 
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(kChunkThreads, 7)
   uint4* buf = exchange[threadIdx.x >> 5];
   const int k = find_entry(t.first, t.count, blockIdx.x);
   const AdamEntry8& e = t.e[k];
-  const StepCoef8 c = load_coef8(t.groups[(e.word >> 3) & 15], t.grad_scale, t.one, t.place_key);
+  const StepCoef8 c = load_coef8(t, e.word);
   const int chunk = (int)blockIdx.x - t.first[k];
   switch (e.word & 3) {
     case CS_F32: step_warp8<float>(e, c, chunk, t.shift, buf); break;
@@ -773,22 +778,28 @@ __global__ void __launch_bounds__(kChunkThreads)
 
 // ---------------------------------------------------------------------------
 // Bias corrections and rounding keys from device step counters: thread i
-// advances group i's counter and writes {1/(1-b1^t), 1/sqrt(1-b2^t), key}.
-struct AdvanceArgs {
+// advances counter i and writes {1/(1-b1^t), 1/sqrt(1-b2^t), key} of its group.
+template <int N>
+struct CountTable {
   int count;
   uint32_t seed;
   float* coef;
-  int64_t* step[CS_ADAMW_MAX_GROUPS];
   double b1[CS_ADAMW_MAX_GROUPS], b2[CS_ADAMW_MAX_GROUPS];
+  int64_t* step[N];
+  uint8_t group[N];
 };
+constexpr int kCountThreads = 64;
 
-__global__ void adamw_advance_kernel(const __grid_constant__ AdvanceArgs a) {
-  const int i = threadIdx.x;
+template <int N>
+__global__ void __launch_bounds__(kCountThreads)
+    adamw_advance_kernel(const __grid_constant__ CountTable<N> a) {
+  const int i = blockIdx.x * kCountThreads + threadIdx.x;
   if (i >= a.count) return;
+  const int g = a.group[i];
   const int64_t t = *a.step[i] + 1;
   *a.step[i] = t;
-  a.coef[4 * i] = (float)(1.0 / (1.0 - pow(a.b1[i], (double)t)));
-  a.coef[4 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2[i], (double)t)));
+  a.coef[4 * i] = (float)(1.0 / (1.0 - pow(a.b1[g], (double)t)));
+  a.coef[4 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(a.b2[g], (double)t)));
   a.coef[4 * i + 2] = __uint_as_float(step_key(a.seed, (uint32_t)t));
 }
 
@@ -1063,11 +1074,11 @@ inline bool aligned_to(const void* q, int bytes) {
 
 struct GroupBuilder {
   AdamGroup g[CS_ADAMW_MAX_GROUPS];
-  int fill(const cs_adamw_group* groups, int n, const float* coef, uint32_t seed) {
+  int fill(const cs_adamw_group* groups, int n, bool counted, uint32_t seed) {
     for (int i = 0; i < n; ++i) {
       const cs_adamw_group& s = groups[i];
       if (!(s.beta1 >= 0.0 && s.beta1 < 1.0 && s.beta2 >= 0.0 && s.beta2 < 1.0)) return CS_ERR_ARG;
-      if (!coef && s.step < 1) return CS_ERR_ARG;
+      if (!counted && s.step < 1) return CS_ERR_ARG;
       AdamGroup& d = g[i];
       d.b1 = (float)s.beta1;
       d.omb1 = (float)(1.0 - s.beta1);
@@ -1077,10 +1088,9 @@ struct GroupBuilder {
       d.lr = (float)s.lr;
       d.wd = (float)s.weight_decay;
       d.lr_dev = s.lr_device;
-      d.coef = coef ? coef + 4 * i : nullptr;
       d.ibc1 = d.rbc2 = 0.0f;
       d.key = 0;
-      if (!coef) {
+      if (!counted) {
         d.ibc1 = (float)(1.0 / (1.0 - std::pow(s.beta1, (double)s.step)));
         d.rbc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(s.beta2, (double)s.step)));
         d.key = step_key(seed, (uint32_t)s.step);
@@ -1157,16 +1167,27 @@ struct RunMoments8 {
   }
 };
 
+// What a table holds beside its tensors.
+struct Common {
+  const AdamGroup* groups;  // CS_ADAMW_MAX_GROUPS, or NULL
+  const float* coef;
+  bool each;
+  int first_place;
+  const float* grad_scale;
+};
+
 // Packs tensors (empty ones left out) into tables of at most N entries and
 // launches each full one.
 template <class Run, class Entry, int N>
-int launch_tables(const cs_adamw_tensor* tensors, int count, int first_place, const AdamGroup* g,
-                  const float* grad_scale, cudaStream_t st) {
+int launch_tables(const cs_adamw_tensor* tensors, int count, const Common& c, cudaStream_t st) {
   Table<Entry, N> t;
   t.one = 1.0f;
-  t.place_key = place_key((uint32_t)first_place);
-  t.grad_scale = grad_scale;
-  for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) t.groups[i] = g ? g[i] : AdamGroup{};
+  t.place_key = place_key((uint32_t)c.first_place);
+  t.grad_scale = c.grad_scale;
+  t.coef = c.coef;
+  t.each = c.each;
+  for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i)
+    t.groups[i] = c.groups ? c.groups[i] : AdamGroup{};
   int64_t total = 0;
   bool half = false;
   for (int i = 0; i < count; ++i) {
@@ -1225,25 +1246,71 @@ inline int check_tensors(const cs_adamw_tensor* tensors, int count, int groups, 
 
 // A call of few tensors takes a small table (its parameters stay below 4 KB).
 template <class Run, class Entry, int kSmall, int kLarge>
-int run_tables(const cs_adamw_tensor* tensors, int count, int first_place, const AdamGroup* g,
-               const float* grad_scale, cudaStream_t st) {
+int run_tables(const cs_adamw_tensor* tensors, int count, const Common& c, cudaStream_t st) {
   static_assert(sizeof(Table<Entry, kLarge>) <= 32764, "kernel parameter limit");
-  if (count <= kSmall)
-    return launch_tables<Run, Entry, kSmall>(tensors, count, first_place, g, grad_scale, st);
-  return launch_tables<Run, Entry, kLarge>(tensors, count, first_place, g, grad_scale, st);
+  if (count <= kSmall) return launch_tables<Run, Entry, kSmall>(tensors, count, c, st);
+  return launch_tables<Run, Entry, kLarge>(tensors, count, c, st);
 }
 
+// Advances `count` device counters; that of tensor i belongs to group of(i).
+template <int N, class Of>
+int launch_advance(int64_t* const* steps, int count, const Of& of, const cs_adamw_group* groups,
+                   int num_groups, uint32_t seed, float* coef, cudaStream_t st) {
+  CountTable<N> a;
+  a.seed = seed;
+  for (int i = 0; i < CS_ADAMW_MAX_GROUPS; ++i) {
+    a.b1[i] = i < num_groups ? groups[i].beta1 : 0.0;
+    a.b2[i] = i < num_groups ? groups[i].beta2 : 0.0;
+  }
+  for (int at = 0; at < count; at += N) {
+    a.count = count - at < N ? count - at : N;
+    a.coef = coef + 4 * (int64_t)at;
+    for (int i = 0; i < a.count; ++i) {
+      a.step[i] = steps[at + i];
+      a.group[i] = (uint8_t)of(at + i);
+    }
+    adamw_advance_kernel<N>
+        <<<(a.count + kCountThreads - 1) / kCountThreads, kCountThreads, 0, st>>>(a);
+    if (int rc = launch_status()) return rc;
+  }
+  return CS_OK;
+}
+
+// Counters of a launch.  The large table stays below 4 KB: a launch with 4 KB of
+// parameters takes the host 2.3 us, with 32 KB 5.4.
+constexpr int kCountSmall = 16, kCountLarge = 400;
+static_assert(sizeof(CountTable<kCountLarge>) <= 4096, "a short launch");
+
+// A step counted on the host, by device counters of the groups (coef, which
+// cs_adamw_advance wrote), or by one of each tensor (steps, which are advanced
+// here; work holds what they give).
 template <class Run, class Entry, int kSmall, int kLarge>
 int step_entry(const cs_adamw_tensor* tensors, int count, const cs_adamw_group* groups,
-               int num_groups, const float* coef, uint32_t seed, int first_place,
-               const float* grad_scale, void* stream) {
+               int num_groups, int64_t* const* steps, float* work, const float* coef,
+               uint32_t seed, int first_place, const float* grad_scale, void* stream) {
   if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups || first_place < 0)
     return CS_ERR_ARG;
   if (int rc = check_tensors(tensors, count, num_groups, Run::kMomentBytes)) return rc;
+  if (steps) {
+    if (!work || !aligned_to(work, 4)) return CS_ERR_ARG;
+    for (int i = 0; i < count; ++i)
+      if (!steps[i] || !aligned_to(steps[i], 8)) return CS_ERR_ARG;
+    coef = work;
+  }
   GroupBuilder b;
-  if (int rc = b.fill(groups, num_groups, coef, seed)) return rc;
-  return run_tables<Run, Entry, kSmall, kLarge>(tensors, count, first_place, b.g, grad_scale,
-                                                (cudaStream_t)stream);
+  if (int rc = b.fill(groups, num_groups, coef != nullptr, seed)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (steps) {
+    const auto of = [tensors](int i) { return tensors[i].group; };
+    const int rc = count <= kCountSmall
+                       ? launch_advance<kCountSmall>(steps, count, of, groups, num_groups, seed,
+                                                     work, st)
+                       : launch_advance<kCountLarge>(steps, count, of, groups, num_groups, seed,
+                                                     work, st);
+    if (rc) return rc;
+  }
+  return run_tables<Run, Entry, kSmall, kLarge>(
+      tensors, count, Common{b.g, coef, steps != nullptr, first_place, grad_scale}, st);
 }
 
 template <int N>
@@ -1329,15 +1396,24 @@ extern "C" {
 
 int cs_adamw_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
                   int32_t num_groups, const float* coef, const float* grad_scale, void* stream) {
-  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, coef, 0, 0,
-                                                 grad_scale, stream);
+  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, nullptr,
+                                                 nullptr, coef, 0, 0, grad_scale, stream);
+}
+
+int cs_adamw_step_counted(const cs_adamw_tensor* tensors, int32_t count,
+                          const cs_adamw_group* groups, int32_t num_groups, int64_t* const* steps,
+                          float* workspace, const float* grad_scale, void* stream) {
+  if (!steps) return CS_ERR_ARG;
+  return step_entry<RunStep, AdamEntry, 40, 560>(tensors, count, groups, num_groups, steps,
+                                                 workspace, nullptr, 0, 0, grad_scale, stream);
 }
 
 int cs_adamw8_step_at(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
                       int32_t num_groups, const float* coef, uint32_t seed, int32_t first_place,
                       const float* grad_scale, void* stream) {
-  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, coef, seed,
-                                                   first_place, grad_scale, stream);
+  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, nullptr,
+                                                   nullptr, coef, seed, first_place, grad_scale,
+                                                   stream);
 }
 
 int cs_adamw8_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw_group* groups,
@@ -1346,32 +1422,36 @@ int cs_adamw8_step(const cs_adamw_tensor* tensors, int32_t count, const cs_adamw
   return cs_adamw8_step_at(tensors, count, groups, num_groups, coef, seed, 0, grad_scale, stream);
 }
 
+int cs_adamw8_step_counted(const cs_adamw_tensor* tensors, int32_t count,
+                           const cs_adamw_group* groups, int32_t num_groups, int64_t* const* steps,
+                           float* workspace, uint32_t seed, int32_t first_place,
+                           const float* grad_scale, void* stream) {
+  if (!steps) return CS_ERR_ARG;
+  return step_entry<RunStep8, AdamEntry8, 36, 420>(tensors, count, groups, num_groups, steps,
+                                                   workspace, nullptr, seed, first_place,
+                                                   grad_scale, stream);
+}
+
 int cs_adamw8_moments(const cs_adamw_tensor* tensors, int32_t count, void* stream) {
   if (int rc = check_tensors(tensors, count, 1, RunMoments8::kMomentBytes)) return rc;
   for (int i = 0; i < count; ++i)
     if (tensors[i].dtype != CS_F32) return CS_ERR_ARG;
-  return run_tables<RunMoments8, AdamEntry8, 36, 420>(tensors, count, 0, nullptr, nullptr,
-                                                      (cudaStream_t)stream);
+  return run_tables<RunMoments8, AdamEntry8, 36, 420>(
+      tensors, count, Common{nullptr, nullptr, false, 0, nullptr}, (cudaStream_t)stream);
 }
 
 int cs_adamw_advance(int64_t* const* steps, const cs_adamw_group* groups, int32_t num_groups,
                      uint32_t seed, float* coef, void* stream) {
   if (!steps || !groups || !coef || num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS)
     return CS_ERR_ARG;
-  AdvanceArgs a{};
-  a.count = num_groups;
-  a.seed = seed;
-  a.coef = coef;
   for (int i = 0; i < num_groups; ++i) {
     if (!steps[i]) return CS_ERR_ARG;
     for (int j = 0; j < i; ++j)
       if (steps[j] == steps[i]) return CS_ERR_ARG;  // each counter advances once
-    a.step[i] = steps[i];
-    a.b1[i] = groups[i].beta1;
-    a.b2[i] = groups[i].beta2;
   }
-  adamw_advance_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(a);
-  return launch_status();
+  static_assert(CS_ADAMW_MAX_GROUPS <= kCountSmall, "one launch");
+  return launch_advance<kCountSmall>(steps, num_groups, [](int i) { return i; }, groups,
+                                     num_groups, seed, coef, (cudaStream_t)stream);
 }
 
 size_t cs_grad_norm_workspace_size(const cs_grad_tensor* tensors, int32_t count) {

@@ -118,6 +118,7 @@ const char* takes_float(at::ScalarType t) {
 }
 const char* takes_float32(at::ScalarType t) { return t == at::kFloat ? nullptr : "Float"; }
 const char* takes_byte(at::ScalarType t) { return t == at::kByte ? nullptr : "Byte"; }
+const char* takes_long(at::ScalarType t) { return t == at::kLong ? nullptr : "Long"; }
 
 void same_length(const TensorList& a, const TensorList& b) {
   if (a.n != b.n)
@@ -278,6 +279,32 @@ std::optional<Tensor> advance(const Groups& r, uint32_t seed, const at::Device& 
   return coef;
 }
 
+// Device step counters of every tensor of a call, where the call has them.
+struct Counters {
+  std::optional<TensorList> list;
+  std::vector<int64_t*> at;
+  Counters(const py::object& seq, const TensorList& params, const Groups& r) {
+    if (seq.is_none()) return;
+    if (!r.counters.empty()) bad("steps are counted by group or by tensor, not by both");
+    list.emplace(seq, "steps");
+    same_length(params, *list);
+    at.reserve(params.n);
+  }
+  size_t size() const { return list ? (size_t)list->n : 0; }
+  void read(Py_ssize_t i, const at::Device& dev, std::vector<Impl*>& changed, Written& written) {
+    if (!list) return;
+    Impl* x = list->get(i, dev, takes_long);
+    if (x->numel() != 1) bad(list->at(i) + " must be one value");
+    changed.push_back(x);
+    at.push_back(static_cast<int64_t*>(list->data(x)));
+    written.add(at.back(), *list, i);
+  }
+  // What the counters give, 16 bytes each.
+  Tensor workspace(const at::Device& dev) const {
+    return at::empty({4 * (int64_t)at.size()}, at::TensorOptions().dtype(at::kFloat).device(dev));
+  }
+};
+
 // Tensors that a call has written: their versions go up once it is enqueued, so
 // that a graph which saved them notices.
 void bump_versions(const std::vector<Impl*>& changed) {
@@ -322,7 +349,7 @@ void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
 
 void adamw_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
                 const py::object& exp_avg_sqs_, const py::list& groups,
-                const std::optional<Tensor>& grad_scale) {
+                const std::optional<Tensor>& grad_scale, const py::object& steps) {
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       v(exp_avg_sqs_, "exp_avg_sqs");
   for (const TensorList* l : {&grads, &m, &v}) same_length(params, *l);
@@ -336,8 +363,9 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
   std::vector<Impl*> changed = r.changed;
-  changed.reserve(changed.size() + 3 * params.n);
-  Written written(3 * params.n);
+  Counters counters(steps, params, r);
+  changed.reserve(changed.size() + counters.size() + 3 * params.n);
+  Written written(counters.size() + 3 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
     Impl* p;
@@ -346,6 +374,7 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     Impl* vi = v.get(i, dev, takes_float32);
     check_like(mi, p, contiguous, m, i);
     check_like(vi, p, contiguous, v, i);
+    counters.read(i, dev, changed, written);
     if (!s.numel) continue;
     changed.push_back(mi);
     changed.push_back(vi);
@@ -353,18 +382,27 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     written.add(s.exp_avg_sq = v.data(vi), v, i);
   }
   set_groups(r, t);
-  const std::optional<Tensor> coef = advance(r, 0, dev);
-  check(cs_adamw_step(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                      coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
-                      stream_of(dev)),
-        "cs_adamw_step");
+  if (counters.list) {
+    const Tensor work = counters.workspace(dev);
+    check(cs_adamw_step_counted(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
+                                counters.at.data(), static_cast<float*>(work.data_ptr()), scale,
+                                stream_of(dev)),
+          "cs_adamw_step_counted");
+  } else {
+    const std::optional<Tensor> coef = advance(r, 0, dev);
+    check(cs_adamw_step(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
+                        coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
+                        stream_of(dev)),
+          "cs_adamw_step");
+  }
   bump_versions(changed);
 }
 
 void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
                  const py::object& m_scales_, const py::object& exp_avg_sqs_,
                  const py::object& v_scales_, const py::list& groups, uint32_t seed,
-                 const std::optional<Tensor>& grad_scale, int32_t first_place) {
+                 const std::optional<Tensor>& grad_scale, int32_t first_place,
+                 const py::object& steps) {
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       ms(m_scales_, "exp_avg_scales"), v(exp_avg_sqs_, "exp_avg_sqs"),
       vs(v_scales_, "exp_avg_sq_scales");
@@ -379,8 +417,9 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
   std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
   std::vector<Tensor> copies;
   std::vector<Impl*> changed = r.changed;
-  changed.reserve(changed.size() + 5 * params.n);
-  Written written(5 * params.n);
+  Counters counters(steps, params, r);
+  changed.reserve(changed.size() + counters.size() + 5 * params.n);
+  Written written(counters.size() + 5 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     cs_adamw_tensor& s = t[i];
     Impl* p;
@@ -393,6 +432,7 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
     Impl* vsi = vs.get(i, dev, takes_byte);
     check_scales(msi, scale_count(s.numel), ms, i);
     check_scales(vsi, scale_count(s.numel), vs, i);
+    counters.read(i, dev, changed, written);
     if (!s.numel) continue;
     for (Impl* x : {mi, vi, msi, vsi}) changed.push_back(x);
     written.add(s.exp_avg = m.data(mi), m, i);
@@ -401,11 +441,19 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
     written.add(s.exp_avg_sq_scales = static_cast<uint8_t*>(vs.data(vsi)), vs, i);
   }
   set_groups(r, t);
-  const std::optional<Tensor> coef = advance(r, seed, dev);
-  check(cs_adamw8_step_at(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                          coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed,
-                          first_place, scale, stream_of(dev)),
-        "cs_adamw8_step_at");
+  if (counters.list) {
+    const Tensor work = counters.workspace(dev);
+    check(cs_adamw8_step_counted(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
+                                 counters.at.data(), static_cast<float*>(work.data_ptr()), seed,
+                                 first_place, scale, stream_of(dev)),
+          "cs_adamw8_step_counted");
+  } else {
+    const std::optional<Tensor> coef = advance(r, seed, dev);
+    check(cs_adamw8_step_at(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
+                            coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed,
+                            first_place, scale, stream_of(dev)),
+          "cs_adamw8_step_at");
+  }
   bump_versions(changed);
 }
 

@@ -37,3 +37,29 @@ def test_a_first_place_below_zero_is_refused():
         t[0] = tensor
         assert nat.call("cs_adamw8_step_at", ctypes.addressof(t), 1, ctypes.addressof(g), 1, None,
                         7, place, None, None) == want
+
+
+@pytest.mark.parametrize("name", ["cs_adamw_step_counted", "cs_adamw8_step_counted"])
+def test_counted_steps_refuse_missing_counters_and_workspaces(name):
+    t = (CTensor * 600)(*[_tensor() for _ in range(600)])
+    g = (type(_group()) * 1)(_group(step=0))  # the host's count is not read
+    good = [256 + 8 * i for i in range(600)]
+
+    def call(steps, work=4096, count=600, place=0):
+        steps = steps and (ctypes.c_void_p * 600)(*steps)
+        args = [ctypes.addressof(t), count, ctypes.addressof(g), 1,
+                steps and ctypes.addressof(steps), work]
+        if name == "cs_adamw8_step_counted":
+            args += [7, place]
+        return nat.call(name, *args, None, None)
+    assert call(good[:-1] + [None]) == CS_ERR_ARG
+    assert call(good[:-1] + [260]) == CS_ERR_ARG
+    assert call(None) == CS_ERR_ARG
+    assert call(good, work=None) == CS_ERR_ARG
+    assert call(good, work=4098) == CS_ERR_ARG
+    assert call(good, count=-1) == CS_ERR_ARG
+    assert call(good, count=0) == CS_OK
+    if name == "cs_adamw8_step_counted":
+        assert call(good, place=-1) == CS_ERR_ARG
+    t[599].exp_avg = None
+    assert call(good) == CS_ERR_ARG

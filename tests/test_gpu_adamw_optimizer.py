@@ -121,3 +121,72 @@ def test_groups_may_differ_in_capturable(bits):
             opt.step()
         runs.append([x for p in ps for x in (p, *opt.moments(p))])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_parameter_without_a_gradient_is_not_counted(bits):
+    """The second parameter has a gradient in steps 1, 2 and 5 only, the third from
+    step 3 on, but not in 4: counts on the device and on the host agree, and so do
+    parameters and moments, bit for bit."""
+    runs = []
+    for capturable in (False, True):
+        ps, gen = params_of((3000, 257, 700), seed=4)
+        opt = manbo.AdamW(ps, lr=0.01, state_bits=bits, capturable=capturable, seed=3)
+        for t in range(1, 6):
+            here = (True, t in (1, 2, 5), t in (3, 5))
+            for p, yes in zip(ps, here):
+                g = make(p.numel(), F32, gen)
+                p.grad = g if yes else None
+            before = n64(ps[1]), opt.moments(ps[1]) if t > 1 else None
+            opt.step()
+            if t == 5:  # its third step
+                (m, v), now = before[1], ps[1]
+                want = oa.adamw64(before[0], n64(now.grad), n64(m), n64(v), 3, lr=0.01)
+                assert (np.abs(n64(now) - want[0]) <= 2 * want[3][0]).all()
+        assert [int(opt.state[p]["step"]) for p in ps] == [5, 3, 2]
+        runs.append([x for p in ps for x in (p, *opt.moments(p))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_captured_step_counts_its_own_parameters_only(bits):
+    """Captured while the second parameter has no gradient, replayed twice, then
+    an eager step of both, then a replay: as eager steps without a graph."""
+    runs = []
+    for captured in (False, True):
+        ps, gen = params_of((3000, 257), seed=5)
+        for p in ps:
+            p.grad = make(p.numel(), F32, gen)
+        grads = [p.grad for p in ps]
+        opt = manbo.AdamW(ps, lr=0.01, state_bits=bits, capturable=True, max_grad_norm=0.1)
+        opt.step()
+        ps[1].grad = None
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                opt.step()
+        for both in (False, False, True, False):
+            ps[1].grad = grads[1] if both else None
+            graph.replay() if captured and not both else opt.step()
+        assert [int(opt.state[p]["step"]) for p in ps] == [5, 2]
+        runs.append([x for p in ps for x in (p, *opt.moments(p))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("count", [1, 130, 1300])
+def test_counts_of_many_parameters(count):
+    """Counters on the device through every table size, each at another step."""
+    runs = []
+    for capturable in (False, True):
+        ps, gen = params_of([1 + i % 37 for i in range(count)], seed=count)
+        opt = manbo.AdamW(ps, lr=0.01, capturable=capturable)
+        for t in range(4):
+            for i, p in enumerate(ps):
+                p.grad = make(p.numel(), F32, gen)
+                if i % 4 < t:
+                    p.grad = None
+            if any(p.grad is not None for p in ps):
+                opt.step()
+        assert [int(opt.state[p]["step"]) for p in ps] == [1 + i % 4 for i in range(count)]
+        runs.append([x for p in ps for x in (p, *opt.moments(p))])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
