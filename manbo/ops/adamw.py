@@ -49,7 +49,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     """
     _ext.load().adamw_step(params, grads, exp_avgs, exp_avg_sqs,
                            [(len(params), lr, betas[0], betas[1], eps, weight_decay, step)],
-                           grad_scale, None)
+                           grad_scale)
 
 
 def adamw8_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
@@ -76,7 +76,7 @@ def adamw8_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     _ext.load().adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs,
                             exp_avg_sq_scales,
                             [(len(params), lr, betas[0], betas[1], eps, weight_decay, step)],
-                            seed & 0xFFFFFFFF, grad_scale, 0, None)
+                            seed & 0xFFFFFFFF, grad_scale)
 
 
 def adamw8_state(param: torch.Tensor) -> Tuple[torch.Tensor, ...]:

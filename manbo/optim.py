@@ -241,13 +241,13 @@ class AdamW(Optimizer):
         plan = self._plan()
         if not plan:
             return loss
-        scale = None
+        norm = scale = None
         if self.defaults["max_grad_norm"] > 0:
             if len({device for device, *_ in plan}) > 1:
                 raise ValueError("max_grad_norm needs every parameter on one device")
             grads = [g for parts in plan.values() for part in parts for g in part[3]]
-            self.grad_norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
-        ext = _ext.load()
+            norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
+        calls, counted = [], []
         places = {}  # 8-bit parameters already stepped with a seed, which draw other bits
         for (_, bits, seed, capturable), parts in plan.items():
             for at in range(0, len(parts), _ADAMW_MAX_GROUPS):
@@ -255,23 +255,31 @@ class AdamW(Optimizer):
                 groups = [(len(ps), g["lr"], g["betas"][0], g["betas"][1], g["eps"],
                            g["weight_decay"], 1 if capturable else step + 1)
                           for g, step, ps, _, _ in some]
-                params, grads, states = ([x for part in some for x in part[k]] for k in (2, 3, 4))
-                m, v = ([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq"))
+                if len(some) == 1:
+                    params, grads, states = some[0][2:]
+                else:
+                    params, grads, states = ([x for part in some for x in part[k]]
+                                             for k in (2, 3, 4))
+                m = [s["exp_avg"] for s in states]
+                v = [s["exp_avg_sq"] for s in states]
                 steps = [s["step"] for s in states] if capturable else None
                 if bits == 8:
-                    ms, vs = ([s[k] for s in states]
-                              for k in ("exp_avg_scales", "exp_avg_sq_scales"))
+                    ms = [s["exp_avg_scales"] for s in states]
+                    vs = [s["exp_avg_sq_scales"] for s in states]
                     seed &= 0xFFFFFFFF
                     first = places.get(seed, 0)
                     places[seed] = first + len(params)
-                    ext.adamw8_step(params, grads, m, ms, v, vs, groups, seed, scale, first,
-                                    steps)
+                    calls.append((params, grads, m, v, groups, steps, ms, vs, seed, first))
                 else:
-                    ext.adamw_step(params, grads, m, v, groups, scale, steps)
+                    calls.append((params, grads, m, v, groups, steps))
                 if not capturable:
-                    for _, step, _, _, sts in some:
-                        for st in sts:
-                            st["step"] = step + 1
+                    counted += some
+        _ext.load().adamw_steps(calls, scale)  # all are checked before one runs
+        if norm is not None:
+            self.grad_norm = norm
+        for _, step, _, _, states in counted:
+            for st in states:
+                st["step"] = step + 1
         return loss
 
     @torch.no_grad()

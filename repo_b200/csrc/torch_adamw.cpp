@@ -283,7 +283,7 @@ std::optional<Tensor> advance(const Groups& r, uint32_t seed, const at::Device& 
 struct Counters {
   std::optional<TensorList> list;
   std::vector<int64_t*> at;
-  Counters(const py::object& seq, const TensorList& params, const Groups& r) {
+  Counters(const py::handle& seq, const TensorList& params, const Groups& r) {
     if (seq.is_none()) return;
     if (!r.counters.empty()) bad("steps are counted by group or by tensor, not by both");
     list.emplace(seq, "steps");
@@ -298,10 +298,6 @@ struct Counters {
     changed.push_back(x);
     at.push_back(static_cast<int64_t*>(list->data(x)));
     written.add(at.back(), *list, i);
-  }
-  // What the counters give, 16 bytes each.
-  Tensor workspace(const at::Device& dev) const {
-    return at::empty({4 * (int64_t)at.size()}, at::TensorOptions().dtype(at::kFloat).device(dev));
   }
 };
 
@@ -347,83 +343,122 @@ void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
   }
 }
 
-void adamw_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
-                const py::object& exp_avg_sqs_, const py::list& groups,
-                const std::optional<Tensor>& grad_scale, const py::object& steps) {
+// A step that has been read and checked and is not yet enqueued.  The caller keeps
+// its tensors.
+struct Step {
+  at::Device dev = at::kCPU;
+  int bits;
+  Groups r;
+  std::vector<cs_adamw_tensor> t;
+  std::vector<Tensor> copies;
+  std::vector<int64_t*> counters;  // one of each tensor, or empty
+  std::vector<Impl*> changed;
+  const float* scale;
+  uint32_t seed = 0;
+  int32_t first_place = 0;
+
+  void enqueue() const {
+    if (t.empty()) return;
+    c10::cuda::CUDAGuard guard(dev);
+    const auto count = (int32_t)t.size(), groups = (int32_t)r.g.size();
+    if (!counters.empty()) {
+      const Tensor work =
+          at::empty({4 * (int64_t)count}, at::TensorOptions().dtype(at::kFloat).device(dev));
+      auto* w = static_cast<float*>(work.data_ptr());
+      if (bits == 8)
+        check(cs_adamw8_step_counted(t.data(), count, r.g.data(), groups, counters.data(), w, seed,
+                                     first_place, scale, stream_of(dev)),
+              "cs_adamw8_step_counted");
+      else
+        check(cs_adamw_step_counted(t.data(), count, r.g.data(), groups, counters.data(), w, scale,
+                                    stream_of(dev)),
+              "cs_adamw_step_counted");
+    } else {
+      const std::optional<Tensor> coef = advance(r, seed, dev);
+      const float* c = coef ? static_cast<const float*>(coef->data_ptr()) : nullptr;
+      if (bits == 8)
+        check(cs_adamw8_step_at(t.data(), count, r.g.data(), groups, c, seed, first_place, scale,
+                                stream_of(dev)),
+              "cs_adamw8_step_at");
+      else
+        check(cs_adamw_step(t.data(), count, r.g.data(), groups, c, scale, stream_of(dev)),
+              "cs_adamw_step");
+    }
+    bump_versions(changed);
+  }
+};
+
+Step read_step(const py::handle& params_, const py::handle& grads_, const py::handle& exp_avgs_,
+               const py::handle& exp_avg_sqs_, const py::list& groups,
+               const std::optional<Tensor>& grad_scale, const py::handle& steps) {
+  Step step;
+  step.bits = 32;
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       v(exp_avg_sqs_, "exp_avg_sqs");
   for (const TensorList* l : {&grads, &m, &v}) same_length(params, *l);
   grads.lazy = true;
-  if (params.n == 0) return;
-  const Groups r = read_groups(groups, params.n, params[0].device());
-  const at::Device dev = device_of(params);
+  if (params.n == 0) return step;
+  step.r = read_groups(groups, params.n, params[0].device());
+  const at::Device dev = step.dev = device_of(params);
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
-  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
-  std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
-  std::vector<Tensor> copies;
-  std::vector<Impl*> changed = r.changed;
-  Counters counters(steps, params, r);
-  changed.reserve(changed.size() + counters.size() + 3 * params.n);
+  step.scale = device_scalar(grad_scale, dev, "grad_scale");
+  step.t.resize(params.n, cs_adamw_tensor{});
+  step.changed = step.r.changed;
+  Counters counters(steps, params, step.r);
+  step.changed.reserve(step.changed.size() + counters.size() + 3 * params.n);
   Written written(counters.size() + 3 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
-    cs_adamw_tensor& s = t[i];
+    cs_adamw_tensor& s = step.t[i];
     Impl* p;
-    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, changed, written);
+    const bool contiguous =
+        read_param(params, grads, i, dev, s, p, step.copies, step.changed, written);
     Impl* mi = m.get(i, dev, takes_float32);
     Impl* vi = v.get(i, dev, takes_float32);
     check_like(mi, p, contiguous, m, i);
     check_like(vi, p, contiguous, v, i);
-    counters.read(i, dev, changed, written);
+    counters.read(i, dev, step.changed, written);
     if (!s.numel) continue;
-    changed.push_back(mi);
-    changed.push_back(vi);
+    step.changed.push_back(mi);
+    step.changed.push_back(vi);
     written.add(s.exp_avg = m.data(mi), m, i);
     written.add(s.exp_avg_sq = v.data(vi), v, i);
   }
-  set_groups(r, t);
-  if (counters.list) {
-    const Tensor work = counters.workspace(dev);
-    check(cs_adamw_step_counted(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                                counters.at.data(), static_cast<float*>(work.data_ptr()), scale,
-                                stream_of(dev)),
-          "cs_adamw_step_counted");
-  } else {
-    const std::optional<Tensor> coef = advance(r, 0, dev);
-    check(cs_adamw_step(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                        coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, scale,
-                        stream_of(dev)),
-          "cs_adamw_step");
-  }
-  bump_versions(changed);
+  set_groups(step.r, step.t);
+  step.counters = std::move(counters.at);
+  return step;
 }
 
-void adamw8_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_,
-                 const py::object& m_scales_, const py::object& exp_avg_sqs_,
-                 const py::object& v_scales_, const py::list& groups, uint32_t seed,
-                 const std::optional<Tensor>& grad_scale, int32_t first_place,
-                 const py::object& steps) {
+Step read_step8(const py::handle& params_, const py::handle& grads_, const py::handle& exp_avgs_,
+                const py::handle& m_scales_, const py::handle& exp_avg_sqs_,
+                const py::handle& v_scales_, const py::list& groups, uint32_t seed,
+                const std::optional<Tensor>& grad_scale, int32_t first_place,
+                const py::handle& steps) {
+  Step step;
+  step.bits = 8;
+  step.seed = seed;
+  step.first_place = first_place;
   TensorList params(params_, "params"), grads(grads_, "grads"), m(exp_avgs_, "exp_avgs"),
       ms(m_scales_, "exp_avg_scales"), v(exp_avg_sqs_, "exp_avg_sqs"),
       vs(v_scales_, "exp_avg_sq_scales");
   for (const TensorList* l : {&grads, &m, &ms, &v, &vs}) same_length(params, *l);
   grads.lazy = true;
-  if (params.n == 0) return;
-  const Groups r = read_groups(groups, params.n, params[0].device());
-  const at::Device dev = device_of(params);
+  if (params.n == 0) return step;
+  step.r = read_groups(groups, params.n, params[0].device());
+  const at::Device dev = step.dev = device_of(params);
   c10::cuda::CUDAGuard guard(dev);
   at::NoGradGuard no_grad;
-  const float* scale = device_scalar(grad_scale, dev, "grad_scale");
-  std::vector<cs_adamw_tensor> t(params.n, cs_adamw_tensor{});
-  std::vector<Tensor> copies;
-  std::vector<Impl*> changed = r.changed;
-  Counters counters(steps, params, r);
-  changed.reserve(changed.size() + counters.size() + 5 * params.n);
+  step.scale = device_scalar(grad_scale, dev, "grad_scale");
+  step.t.resize(params.n, cs_adamw_tensor{});
+  step.changed = step.r.changed;
+  Counters counters(steps, params, step.r);
+  step.changed.reserve(step.changed.size() + counters.size() + 5 * params.n);
   Written written(counters.size() + 5 * params.n);
   for (Py_ssize_t i = 0; i < params.n; ++i) {
-    cs_adamw_tensor& s = t[i];
+    cs_adamw_tensor& s = step.t[i];
     Impl* p;
-    const bool contiguous = read_param(params, grads, i, dev, s, p, copies, changed, written);
+    const bool contiguous =
+        read_param(params, grads, i, dev, s, p, step.copies, step.changed, written);
     Impl* mi = m.get(i, dev, takes_byte);
     Impl* vi = v.get(i, dev, takes_byte);
     check_like(mi, p, contiguous, m, i);
@@ -432,29 +467,50 @@ void adamw8_step(const py::object& params_, const py::object& grads_, const py::
     Impl* vsi = vs.get(i, dev, takes_byte);
     check_scales(msi, scale_count(s.numel), ms, i);
     check_scales(vsi, scale_count(s.numel), vs, i);
-    counters.read(i, dev, changed, written);
+    counters.read(i, dev, step.changed, written);
     if (!s.numel) continue;
-    for (Impl* x : {mi, vi, msi, vsi}) changed.push_back(x);
+    for (Impl* x : {mi, vi, msi, vsi}) step.changed.push_back(x);
     written.add(s.exp_avg = m.data(mi), m, i);
     written.add(s.exp_avg_sq = v.data(vi), v, i);
     written.add(s.exp_avg_scales = static_cast<uint8_t*>(ms.data(msi)), ms, i);
     written.add(s.exp_avg_sq_scales = static_cast<uint8_t*>(vs.data(vsi)), vs, i);
   }
-  set_groups(r, t);
-  if (counters.list) {
-    const Tensor work = counters.workspace(dev);
-    check(cs_adamw8_step_counted(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                                 counters.at.data(), static_cast<float*>(work.data_ptr()), seed,
-                                 first_place, scale, stream_of(dev)),
-          "cs_adamw8_step_counted");
-  } else {
-    const std::optional<Tensor> coef = advance(r, seed, dev);
-    check(cs_adamw8_step_at(t.data(), (int32_t)t.size(), r.g.data(), (int32_t)r.g.size(),
-                            coef ? static_cast<const float*>(coef->data_ptr()) : nullptr, seed,
-                            first_place, scale, stream_of(dev)),
-          "cs_adamw8_step_at");
+  set_groups(step.r, step.t);
+  step.counters = std::move(counters.at);
+  return step;
+}
+
+void adamw_step(const py::object& params, const py::object& grads, const py::object& exp_avgs,
+                const py::object& exp_avg_sqs, const py::list& groups,
+                const std::optional<Tensor>& grad_scale) {
+  read_step(params, grads, exp_avgs, exp_avg_sqs, groups, grad_scale, py::none()).enqueue();
+}
+
+void adamw8_step(const py::object& params, const py::object& grads, const py::object& exp_avgs,
+                 const py::object& m_scales, const py::object& exp_avg_sqs,
+                 const py::object& v_scales, const py::list& groups, uint32_t seed,
+                 const std::optional<Tensor>& grad_scale) {
+  read_step8(params, grads, exp_avgs, m_scales, exp_avg_sqs, v_scales, groups, seed, grad_scale, 0,
+             py::none())
+      .enqueue();
+}
+
+// The calls of one optimiser step: (params, grads, exp_avgs, exp_avg_sqs, groups,
+// steps) each, with 8-bit moments (..., groups, steps, exp_avg_scales,
+// exp_avg_sq_scales, seed, first place); steps is None or the tensors' device
+// counters.  All of them are read and checked before the first is enqueued.
+void adamw_steps(const py::list& calls, const std::optional<Tensor>& grad_scale) {
+  std::vector<Step> all;
+  all.reserve(calls.size());
+  for (const py::handle& call : calls) {
+    const py::tuple c = py::reinterpret_borrow<py::tuple>(call);
+    if (c.size() == 6)
+      all.push_back(read_step(c[0], c[1], c[2], c[3], c[4], grad_scale, c[5]));
+    else
+      all.push_back(read_step8(c[0], c[1], c[2], c[6], c[3], c[7], c[4], c[8].cast<uint32_t>(),
+                               grad_scale, c[9].cast<int32_t>(), c[5]));
   }
-  bump_versions(changed);
+  for (const Step& s : all) s.enqueue();
 }
 
 void adamw8_moments(const py::object& exp_avgs_, const py::object& m_scales_,
@@ -545,6 +601,7 @@ void bind_adamw(py::module_& m) {
   m.attr("ADAMW_MAX_GROUPS") = CS_ADAMW_MAX_GROUPS;
   m.def("adamw_step", &adamw_step);
   m.def("adamw8_step", &adamw8_step);
+  m.def("adamw_steps", &adamw_steps);
   m.def("adamw8_moments", &adamw8_moments);
   m.def("grad_norm", &grad_norm);
 }

@@ -190,3 +190,25 @@ def test_counts_of_many_parameters(count):
         assert [int(opt.state[p]["step"]) for p in ps] == [1 + i % 4 for i in range(count)]
         runs.append([x for p in ps for x in (p, *opt.moments(p))])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_refused_step_moves_no_parameter():
+    """The refusal is in another launch than the first: 8-bit moments after 32-bit
+    ones, the 17th group, a device counter."""
+    def build(n, **kw):
+        ps, gen = params_of((300,) * n, seed=12)
+        for p in ps:
+            p.grad = make(300, F32, gen)
+        return ps
+    for n, groups in ((2, [{}, {"state_bits": 8}]), (20, [{"lr": 1e-3 * i} for i in range(1, 21)]),
+                      (2, [{"capturable": True}, {"capturable": False}])):
+        ps = build(n)
+        opt = manbo.AdamW([{"params": [p], **g} for p, g in zip(ps, groups)])
+        opt.step()
+        old = [[x.clone() for x in (p, *opt.moments(p))] for p in ps]
+        ps[-1].grad = ps[-1].grad.to_sparse()
+        with pytest.raises(ValueError, match="must be a dense tensor"):
+            opt.step()
+        for p, o in zip(ps, old):
+            assert all(torch.equal(a, b) for a, b in zip((p, *opt.moments(p)), o))
+            assert int(opt.state[p]["step"]) == 1
