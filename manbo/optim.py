@@ -137,7 +137,8 @@ class AdamW(Optimizer):
     parameter's layout, 8 as one byte an element with a scale byte for each 256
     elements (see ``manbo.ops.adamw8_step``; ``seed`` feeds its rounding).
     ``max_grad_norm`` > 0 clips by the global norm of all gradients, which stays
-    on the device (``grad_norm`` holds the last one).  Parameters are float32,
+    on the device (``grad_norm`` holds the last one); it is the same in every group,
+    so that it is saved and loaded with them.  Parameters are float32,
     bfloat16 or float16, non-overlapping and dense.
 
     Steps are counted per parameter, those at which it has a gradient.  With
@@ -242,11 +243,14 @@ class AdamW(Optimizer):
         if not plan:
             return loss
         norm = scale = None
-        if self.defaults["max_grad_norm"] > 0:
+        max_norm = self.param_groups[0]["max_grad_norm"]
+        if any(group["max_grad_norm"] != max_norm for group in self.param_groups):
+            raise ValueError("AdamW: max_grad_norm must be the same in every group")
+        if max_norm != 0:
             if len({device for device, *_ in plan}) > 1:
                 raise ValueError("max_grad_norm needs every parameter on one device")
             grads = [g for parts in plan.values() for part in parts for g in part[3]]
-            norm, scale = grad_norm(grads, max_norm=self.defaults["max_grad_norm"])
+            norm, scale = grad_norm(grads, max_norm=max_norm)
         calls, counted = [], []
         places = {}  # 8-bit parameters already stepped with a seed, which draw other bits
         for (_, bits, seed, capturable), parts in plan.items():

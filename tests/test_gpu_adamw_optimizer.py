@@ -212,3 +212,54 @@ def test_a_refused_step_moves_no_parameter():
         for p, o in zip(ps, old):
             assert all(torch.equal(a, b) for a, b in zip((p, *opt.moments(p)), o))
             assert int(opt.state[p]["step"]) == 1
+
+
+def test_a_resumed_optimiser_still_clips():
+    """max_grad_norm is in the saved groups, so it holds after a load, and where a
+    group is given another value."""
+    ps, gen = params_of((700, 50), seed=8)
+    opt = manbo.AdamW(ps, lr=0.01, max_grad_norm=0.05)
+    for p in ps:
+        p.grad = make(p.numel(), F32, gen)
+    opt.step()
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    other = manbo.AdamW(qs)
+    other.load_state_dict(opt.state_dict())
+    for p, q in zip(ps, qs):
+        p.grad = make(p.numel(), F32, gen)
+        q.grad = p.grad.clone()
+    opt.step()
+    other.step()
+    assert torch.equal(opt.grad_norm, other.grad_norm) and float(opt.grad_norm) > 0.05
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    for o in (opt, other):
+        for group in o.param_groups:
+            group["max_grad_norm"] = 0.01 if o is opt else 0.0
+    for q in qs:
+        q.grad = None
+    ps[1].grad = None
+    p, g = ps[0], n64(ps[0].grad)
+    old, (m, v) = n64(p), opt.moments(p)
+    opt.step()
+    _, c = oa.norm64([g], 0.01)
+    want = oa.adamw64(old, g, n64(m), n64(v), 3, lr=0.01, scale=float(np.float32(c)))
+    assert (np.abs(n64(p) - want[0]) <= 2 * want[3][0]).all()
+
+
+def test_groups_that_disagree_on_max_grad_norm_are_refused():
+    ps, gen = params_of((50, 60), seed=8)
+    opt = manbo.AdamW([{"params": ps[:1], "max_grad_norm": 1.0}, {"params": ps[1:]}])
+    for p in ps:
+        p.grad = make(p.numel(), F32, gen)
+    old = [p.clone() for p in ps]
+    with pytest.raises(ValueError, match="max_grad_norm must be the same in every group"):
+        opt.step()
+    assert all(torch.equal(p, o) for p, o in zip(ps, old))
+    for group in opt.param_groups:
+        group["max_grad_norm"] = -1.0
+    with pytest.raises(ValueError, match="Invalid max_norm"):
+        opt.step()
+    for group in opt.param_groups:
+        group["max_grad_norm"] = 1.0
+    opt.step()
+    assert opt.grad_norm is not None
