@@ -13,7 +13,7 @@ gradient norm without reading it back, and can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
-import itertools
+import collections
 import math
 
 import torch
@@ -172,6 +172,8 @@ class AdamW(Optimizer):
         self.grad_norm = None
 
     def __setstate__(self, state):
+        if self.__dict__.get("_loaded") is not None:  # of a load
+            state = {**state, "state": self._loaded}
         super().__setstate__(state)
         self.__dict__.setdefault("grad_norm", None)
         for group in self.param_groups:
@@ -307,34 +309,55 @@ class AdamW(Optimizer):
         """As the base class, except that moments keep their own types (the base
         class casts them to the parameter's) and are copies of the given ones.
         States of ``torch.optim.AdamW`` load too; what this class does not compute
-        (``maximize``, ``amsgrad``, Adam's coupled decay) is refused."""
-        for group in state_dict["param_groups"]:
+        (``maximize``, ``amsgrad``, Adam's coupled decay) is refused.  A refused
+        load changes nothing."""
+        # behind the user's own hooks, so that it sees what they return
+        hook = self.register_load_state_dict_pre_hook(AdamW._take_state)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+            self._loaded = None
+
+    def _take_state(self, state_dict):
+        """Pre-hook of a load: keeps the parameters' new states for ``__setstate__`` and
+        leaves none for the base class to cast."""
+        saved = state_dict["param_groups"]
+        for group in saved:
             if (group.get("maximize") or group.get("amsgrad")
                     or not group.get("decoupled_weight_decay", True)):
                 raise ValueError("AdamW does not support maximize, amsgrad or coupled weight decay")
-        super().load_state_dict({**state_dict, "state": {}})
-        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        own = [(p, g) for g in self.param_groups for p in g["params"]]
-        for i, (p, group) in zip(ids, own):
-            if i not in state_dict["state"]:
-                continue
-            st = {}
-            codes = state_dict["state"][i].get("exp_avg")
-            if codes is not None and codes.dtype == torch.uint8 and codes.stride() != p.stride():
-                raise ValueError("8-bit moments need the strides of the parameter they were "
-                                 "saved with (their blocks follow its storage)")
-            for k, x in state_dict["state"][i].items():
-                if k == "step":
-                    st[k] = int(x)
-                    if group["capturable"]:
-                        st[k] = torch.tensor(st[k], dtype=torch.int64, device=p.device)
-                elif isinstance(x, torch.Tensor):
-                    y = torch.empty_like(p, dtype=x.dtype) if x.shape == p.shape \
-                        else torch.empty_like(x, device=p.device)
-                    st[k] = y.copy_(x)
-                else:
-                    st[k] = x
-            self.state[p] = st
+        if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
+            return None  # which the base class refuses
+        loaded = collections.defaultdict(dict)
+        for group, own in zip(saved, self.param_groups):
+            capturable = group.get("capturable", self.defaults["capturable"])
+            for i, p in zip(group["params"], own["params"]):
+                if i in state_dict["state"]:
+                    loaded[p] = self._own_state(p, state_dict["state"][i], capturable)
+        self._loaded = loaded
+        return {**state_dict, "state": {}}
+
+    @staticmethod
+    def _own_state(p, state, capturable):
+        """Copies of a parameter's saved moments and step count, on its device."""
+        st = {}
+        codes = state.get("exp_avg")
+        if codes is not None and codes.dtype == torch.uint8 and codes.stride() != p.stride():
+            raise ValueError("8-bit moments need the strides of the parameter they were "
+                             "saved with (their blocks follow its storage)")
+        for k, x in state.items():
+            if k == "step":
+                st[k] = int(x)
+                if capturable:
+                    st[k] = torch.tensor(st[k], dtype=torch.int64, device=p.device)
+            elif isinstance(x, torch.Tensor):
+                y = torch.empty_like(p, dtype=x.dtype) if x.shape == p.shape \
+                    else torch.empty_like(x, device=p.device)
+                st[k] = y.copy_(x)
+            else:
+                st[k] = x
+        return st
 
 
 __all__ = ["Adan", "AdamW"]
