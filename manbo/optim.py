@@ -21,7 +21,7 @@ from torch.optim.optimizer import Optimizer
 
 from repo_b200 import _ext
 
-from .ops.adamw import adamw8_moments, adamw8_state, grad_norm
+from .ops.adamw import ADAMW8_BLOCK, adamw8_moments, adamw8_state, grad_norm
 from .ops.optim import adan_step_from_grad_kernel
 
 DEFAULT_TILELANG_THREADS = 256
@@ -128,6 +128,11 @@ class Adan(Optimizer):
 
 
 _ADAMW_MAX_GROUPS = 16  # hyper-parameter groups of one launch
+
+
+def _order(t):
+    """A tensor's strides where they matter: of sizes above 1."""
+    return [s for n, s in zip(t.shape, t.stride()) if n > 1]
 
 
 class AdamW(Optimizer):
@@ -308,9 +313,10 @@ class AdamW(Optimizer):
     def load_state_dict(self, state_dict):
         """As the base class, except that moments keep their own types (the base
         class casts them to the parameter's) and are copies of the given ones.
-        States of ``torch.optim.AdamW`` load too; what this class does not compute
-        (``maximize``, ``amsgrad``, Adam's coupled decay) is refused.  A refused
-        load changes nothing."""
+        States of ``torch.optim.AdamW`` load too, into groups of 32-bit moments;
+        what this class does not compute (``maximize``, ``amsgrad``, Adam's coupled
+        decay) and moments of other ``state_bits`` than the group's are refused.  A
+        refused load changes nothing."""
         # behind the user's own hooks, so that it sees what they return
         hook = self.register_load_state_dict_pre_hook(AdamW._take_state)
         try:
@@ -331,32 +337,50 @@ class AdamW(Optimizer):
             return None  # which the base class refuses
         loaded = collections.defaultdict(dict)
         for group, own in zip(saved, self.param_groups):
-            capturable = group.get("capturable", self.defaults["capturable"])
+            bits, capturable = (group.get(k, self.defaults[k])
+                                for k in ("state_bits", "capturable"))
             for i, p in zip(group["params"], own["params"]):
                 if i in state_dict["state"]:
-                    loaded[p] = self._own_state(p, state_dict["state"][i], capturable)
+                    loaded[p] = self._own_state(p, state_dict["state"][i], bits,
+                                                capturable)
         self._loaded = loaded
         return {**state_dict, "state": {}}
 
     @staticmethod
-    def _own_state(p, state, capturable):
-        """Copies of a parameter's saved moments and step count, on its device."""
+    def _own_state(p, state, bits, capturable):
+        """Copies of a parameter's saved moments and step count, on its device, as a
+        step takes them: 32-bit moments in float32 (torch keeps them in the
+        parameter's type), 8-bit ones as they are."""
+        if not state:
+            return {}
+        names = ("exp_avg", "exp_avg_sq")
+        scales = ("exp_avg_scales", "exp_avg_sq_scales") if bits == 8 else ()
+        missing = [k for k in (*names, *scales, "step") if k not in state]
+        if not all(state[k].dtype == torch.uint8 if bits == 8 else state[k].is_floating_point()
+                   for k in names if k in state):
+            raise ValueError(f"AdamW state is not of state_bits={bits}")
+        if missing:
+            raise ValueError(f"AdamW state lacks {', '.join(missing)}")
+        blocks = -(-p.numel() // ADAMW8_BLOCK)
         st = {}
-        codes = state.get("exp_avg")
-        if codes is not None and codes.dtype == torch.uint8 and codes.stride() != p.stride():
-            raise ValueError("8-bit moments need the strides of the parameter they were "
-                             "saved with (their blocks follow its storage)")
         for k, x in state.items():
-            if k == "step":
-                st[k] = int(x)
-                if capturable:
-                    st[k] = torch.tensor(st[k], dtype=torch.int64, device=p.device)
-            elif isinstance(x, torch.Tensor):
-                y = torch.empty_like(p, dtype=x.dtype) if x.shape == p.shape \
-                    else torch.empty_like(x, device=p.device)
-                st[k] = y.copy_(x)
+            if k in names:
+                if x.shape != p.shape:
+                    raise ValueError(f"{k} must have its parameter's shape")
+                if bits == 8 and _order(x) != _order(p):
+                    raise ValueError("8-bit moments need the strides of the parameter they were "
+                                     "saved with (their blocks follow its storage)")
+                kind = torch.uint8 if bits == 8 else torch.float32
+                st[k] = torch.empty_like(p, dtype=kind).copy_(x)
+            elif k in scales:
+                if x.dtype != torch.uint8 or x.numel() != blocks:
+                    raise ValueError(f"{k} must be {blocks} uint8 scales")
+                st[k] = torch.empty(blocks, dtype=torch.uint8, device=p.device).copy_(x.view(-1))
+            elif k == "step":
+                st[k] = (torch.as_tensor(x).reshape(()).to(p.device, torch.int64, copy=True)
+                         if capturable else int(x))
             else:
-                st[k] = x
+                st[k] = x.to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
         return st
 
 

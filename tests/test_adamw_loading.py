@@ -87,3 +87,76 @@ def test_copies_of_an_optimiser_load_too():
     assert other.state[ps[0]]["step"] == 12
     other.load_state_dict(_saved(other, step=13))
     assert other.state[ps[0]]["step"] == 13 and opt.state[p]["step"] == 12
+
+
+def test_moments_of_16_bit_states_become_float32():
+    p = torch.zeros(4, 6, dtype=torch.bfloat16).t().requires_grad_()
+    opt = manbo.AdamW([p])
+    old = torch.optim.AdamW([p], lr=0.5)
+    p.grad = torch.randn(6, 4).bfloat16()
+    old.step()
+    opt.load_state_dict(old.state_dict())
+    for k in ("exp_avg", "exp_avg_sq"):
+        x = opt.state[p][k]
+        assert x.dtype == torch.float32 and x.stride() == p.stride()
+        assert torch.equal(x, old.state[p][k].float())
+    assert opt.state[p]["step"] == 1 and opt.param_groups[0]["lr"] == 0.5
+
+
+def test_states_that_a_step_could_not_take_are_refused():
+    (p, q), opt = _optimiser()
+    for i, change, msg in (
+            (1, dict(exp_avg=torch.ones(8)), "exp_avg must have its parameter's shape"),
+            (1, dict(exp_avg_sq=torch.ones(7, dtype=torch.uint8)), "state_bits=32"),
+            (1, dict(exp_avg_sq=None), "exp_avg_sq"), (1, dict(step=None), "step"),
+            (0, dict(exp_avg=torch.ones(5, 3)), "state_bits=8"),
+            (0, dict(exp_avg_sq=torch.ones(5, 3)), "state_bits=8"),
+            (0, dict(exp_avg_sq_scales=None), "exp_avg_sq_scales"),
+            (0, dict(exp_avg_scales=torch.ones(2, dtype=torch.uint8)), "1 uint8 scales"),
+            (0, dict(exp_avg_scales=torch.ones(1)), "1 uint8 scales"),
+            (0, dict(exp_avg=torch.ones(3, 5, dtype=torch.uint8)), "parameter's shape")):
+        saved = _saved(opt)
+        for k, x in change.items():
+            if x is None:
+                del saved["state"][i][k]
+            else:
+                saved["state"][i][k] = x
+        with pytest.raises(ValueError, match=msg):
+            opt.load_state_dict(saved)
+        assert not opt.state
+    # a state of 32-bit moments for an optimiser that keeps 8-bit ones
+    old = torch.optim.AdamW([q])
+    q.grad = torch.ones(7)
+    old.step()
+    with pytest.raises(ValueError, match="state_bits=8"):
+        manbo.AdamW([q], state_bits=8).load_state_dict(old.state_dict())
+    opt.load_state_dict({**_saved(opt), "state": {0: {}}})  # empty: as if there were none
+    assert not opt.state[p]
+
+
+def test_strides_of_sizes_of_one_do_not_matter():
+    p = torch.zeros(1, 5).as_strided((1, 5), (1, 1)).requires_grad_()
+    opt = manbo.AdamW([p], state_bits=8)
+    saved = opt.state_dict()
+    codes = torch.arange(5, dtype=torch.uint8).view(1, 5)
+    s = torch.tensor([90], dtype=torch.uint8)
+    saved["state"] = {0: dict(exp_avg=codes, exp_avg_scales=s, exp_avg_sq=codes,
+                              exp_avg_sq_scales=s, step=1)}
+    opt.load_state_dict(saved)
+    assert torch.equal(opt.state[p]["exp_avg"], codes)
+
+
+@pytest.mark.parametrize("step", [3, 3.0, torch.tensor(3.0), torch.tensor([3])])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_step_counts_of_every_kind(step, capturable):
+    p = torch.zeros(7, requires_grad=True)
+    opt = manbo.AdamW([p], capturable=capturable)
+    saved = opt.state_dict()
+    saved["state"] = {0: dict(exp_avg=torch.ones(7), exp_avg_sq=torch.ones(7), step=step)}
+    opt.load_state_dict(saved)
+    got = opt.state[p]["step"]
+    if capturable:
+        assert got.dtype == torch.int64 and got.shape == () and got is not step
+    else:
+        assert type(got) is int
+    assert int(got) == 3
