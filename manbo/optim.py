@@ -307,8 +307,20 @@ class AdamW(Optimizer):
 
     @torch.no_grad()
     def restart_opt(self):
-        """Forget every moment and step count."""
-        self.state.clear()
+        """Zero every moment and step count in place, so that a step captured before
+        goes on from there.  A state made with other ``state_bits`` or ``capturable``
+        than its group has now is dropped."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st:
+                    continue
+                if (("exp_avg_scales" in st) != (group["state_bits"] == 8)
+                        or isinstance(st["step"], torch.Tensor) != bool(group["capturable"])):
+                    del self.state[p]
+                    continue
+                for k, x in st.items():
+                    st[k] = x.zero_() if isinstance(x, torch.Tensor) else 0
 
     def load_state_dict(self, state_dict):
         """As the base class, except that moments keep their own types (the base
@@ -316,7 +328,8 @@ class AdamW(Optimizer):
         States of ``torch.optim.AdamW`` load too, into groups of 32-bit moments;
         what this class does not compute (``maximize``, ``amsgrad``, Adam's coupled
         decay) and moments of other ``state_bits`` than the group's are refused.  A
-        refused load changes nothing."""
+        refused load changes nothing.  A step captured before a load has to be
+        captured again: its moments, counts and hyper-parameters are the old ones."""
         # behind the user's own hooks, so that it sees what they return
         hook = self.register_load_state_dict_pre_hook(AdamW._take_state)
         try:

@@ -293,3 +293,45 @@ def test_state_of_torch_adamw_with_16_bit_parameters_continues(dtype, capturable
         np.testing.assert_array_equal(n64(p)[~ok], want[0][~ok])
         check_param(p.detach()[torch.from_numpy(ok).cuda()], dtype, want[0][ok], want[3][0][ok])
         assert int(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_restart_zeroes_what_a_captured_step_writes(bits):
+    ps, gen = params_of((700, 50), seed=10)
+    opt = manbo.AdamW(ps, lr=0.01, state_bits=bits, capturable=True)
+    for p in ps:
+        p.grad = make(p.numel(), F32, gen)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    kept = [{k: x.data_ptr() for k, x in opt.state[p].items()} for p in ps]
+    opt.restart_opt()
+    for p, k in zip(ps, kept):
+        assert {name: x.data_ptr() for name, x in opt.state[p].items()} == k
+        assert all(not x.any() for x in opt.state[p].values())
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    fresh = manbo.AdamW(qs, lr=0.01, state_bits=bits)
+    for _ in range(2):
+        graph.replay()
+        for p, q in zip(ps, qs):
+            q.grad = p.grad.clone()
+        fresh.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and int(opt.state[p]["step"]) == 2
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(p), fresh.moments(q)))
+
+
+def test_restart_drops_a_state_of_another_kind():
+    ps, gen = params_of((700, 50), seed=10)
+    opt = manbo.AdamW([{"params": [p]} for p in ps], lr=0.01)
+    for p in ps:
+        p.grad = make(p.numel(), F32, gen)
+    opt.step()
+    opt.param_groups[0].update(state_bits=8, capturable=True)
+    opt.restart_opt()
+    assert ps[0] not in opt.state and opt.state[ps[1]]["step"] == 0
+    opt.step()
+    assert opt.state[ps[0]]["exp_avg"].dtype == torch.uint8
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
