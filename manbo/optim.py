@@ -356,8 +356,21 @@ class AdamW(Optimizer):
                 if i in state_dict["state"]:
                     loaded[p] = self._own_state(p, state_dict["state"][i], bits,
                                                 capturable)
+        rates = {}  # groups that shared a tensor go on sharing one
+        groups = []
+        for group, own in zip(saved, self.param_groups):
+            lr = group.get("lr")
+            if isinstance(lr, torch.Tensor):
+                if not group.get("capturable", self.defaults["capturable"]):
+                    lr = float(lr)
+                elif own["params"]:
+                    device = own["params"][0].device
+                    lr = rates.setdefault((id(lr), device),
+                                          lr.detach().to(device, torch.float32, copy=True))
+                group = {**group, "lr": lr}
+            groups.append(group)
         self._loaded = loaded
-        return {**state_dict, "state": {}}
+        return {**state_dict, "state": {}, "param_groups": groups}
 
     @staticmethod
     def _own_state(p, state, bits, capturable):

@@ -160,3 +160,21 @@ def test_step_counts_of_every_kind(step, capturable):
     else:
         assert type(got) is int
     assert int(got) == 3
+
+
+def test_learning_rates_that_are_tensors():
+    ps = [torch.zeros(3, requires_grad=True) for _ in range(3)]
+    rate = torch.tensor(0.25, dtype=torch.float64)
+
+    def groups(**kw):
+        return [{"params": [p], **kw} for p in ps[:2]] + [{"params": ps[2:], "lr": 0.5}]
+    old = manbo.AdamW(groups(lr=rate), capturable=True)
+    new = manbo.AdamW(groups(), capturable=True)
+    new.load_state_dict(old.state_dict())
+    a, b, c = (g["lr"] for g in new.param_groups)
+    assert a is b and a is not rate and a.dtype == torch.float32 and float(a) == 0.25 and c == 0.5
+    # torch takes a tensor without capturable, too
+    new.load_state_dict(torch.optim.AdamW(groups(lr=torch.tensor(0.125)), foreach=False)
+                        .state_dict())
+    assert [g["lr"] for g in new.param_groups] == [0.125, 0.125, 0.5]
+    assert type(new.param_groups[0]["lr"]) is float

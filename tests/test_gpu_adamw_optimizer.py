@@ -335,3 +335,25 @@ def test_restart_drops_a_state_of_another_kind():
     opt.step()
     assert opt.state[ps[0]]["exp_avg"].dtype == torch.uint8
     assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+
+
+def test_a_learning_rate_saved_from_the_device_and_read_on_the_host():
+    """A checkpoint that was read with every tensor on the host continues."""
+    ps, gen = params_of((700, 50), seed=13)
+    opt = manbo.AdamW(ps, lr=torch.tensor(0.01, device="cuda"), capturable=True)
+    for p in ps:
+        p.grad = make(p.numel(), F32, gen)
+    opt.step()
+    saved = opt.state_dict()
+    host = {"param_groups": [{**g, "lr": g["lr"].cpu()} for g in saved["param_groups"]],
+            "state": {i: {k: x.cpu() for k, x in st.items()} for i, st in saved["state"].items()}}
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    other = manbo.AdamW(qs, capturable=True)
+    other.load_state_dict(host)
+    for p, q in zip(ps, qs):
+        q.grad = p.grad.clone()
+    opt.step()
+    other.step()
+    assert other.param_groups[0]["lr"].is_cuda
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and int(other.state[q]["step"]) == 2
