@@ -319,8 +319,11 @@ class AdamW(Optimizer):
                         or isinstance(st["step"], torch.Tensor) != bool(group["capturable"])):
                     del self.state[p]
                     continue
-                for k, x in st.items():
-                    st[k] = x.zero_() if isinstance(x, torch.Tensor) else 0
+                for x in st.values():
+                    if isinstance(x, torch.Tensor):
+                        x.zero_()
+                if not group["capturable"]:
+                    st["step"] = 0
 
     def load_state_dict(self, state_dict):
         """As the base class, except that moments keep their own types (the base
