@@ -1078,7 +1078,7 @@ struct GroupBuilder {
     for (int i = 0; i < n; ++i) {
       const cs_adamw_group& s = groups[i];
       if (!(s.beta1 >= 0.0 && s.beta1 < 1.0 && s.beta2 >= 0.0 && s.beta2 < 1.0)) return CS_ERR_ARG;
-      if (!counted && s.step < 1) return CS_ERR_ARG;
+      if ((!counted && s.step < 1) || !aligned_to(s.lr_device, 4)) return CS_ERR_ARG;
       AdamGroup& d = g[i];
       d.b1 = (float)s.beta1;
       d.omb1 = (float)(1.0 - s.beta1);
@@ -1288,7 +1288,8 @@ template <class Run, class Entry, int kSmall, int kLarge>
 int step_entry(const cs_adamw_tensor* tensors, int count, const cs_adamw_group* groups,
                int num_groups, int64_t* const* steps, float* work, const float* coef,
                uint32_t seed, int first_place, const float* grad_scale, void* stream) {
-  if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups || first_place < 0)
+  if (num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS || !groups || first_place < 0 ||
+      !aligned_to(coef, 4) || !aligned_to(grad_scale, 4))
     return CS_ERR_ARG;
   if (int rc = check_tensors(tensors, count, num_groups, Run::kMomentBytes)) return rc;
   if (steps) {
@@ -1442,10 +1443,11 @@ int cs_adamw8_moments(const cs_adamw_tensor* tensors, int32_t count, void* strea
 
 int cs_adamw_advance(int64_t* const* steps, const cs_adamw_group* groups, int32_t num_groups,
                      uint32_t seed, float* coef, void* stream) {
-  if (!steps || !groups || !coef || num_groups < 1 || num_groups > CS_ADAMW_MAX_GROUPS)
+  if (!steps || !groups || !coef || !aligned_to(coef, 4) || num_groups < 1 ||
+      num_groups > CS_ADAMW_MAX_GROUPS)
     return CS_ERR_ARG;
   for (int i = 0; i < num_groups; ++i) {
-    if (!steps[i]) return CS_ERR_ARG;
+    if (!steps[i] || !aligned_to(steps[i], 8)) return CS_ERR_ARG;
     for (int j = 0; j < i; ++j)
       if (steps[j] == steps[i]) return CS_ERR_ARG;  // each counter advances once
   }
@@ -1466,7 +1468,7 @@ size_t cs_grad_norm_workspace_size(const cs_grad_tensor* tensors, int32_t count)
 int cs_grad_norm(const cs_grad_tensor* tensors, int32_t count, double max_norm, double eps,
                  float* norm, float* scale, void* workspace, void* stream) {
   if (count < 0 || count > kMaxTensors || (count > 0 && !tensors) || !norm ||
-      !aligned_to(workspace, 8))
+      !aligned_to(norm, 4) || !aligned_to(scale, 4) || !aligned_to(workspace, 8))
     return CS_ERR_ARG;
   for (int i = 0; i < count; ++i)
     if (tensors[i].numel < 0 || tensors[i].numel > kMaxNumel || tensors[i].dtype < CS_F32 ||

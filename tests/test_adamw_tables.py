@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from repo_b200 import _native as nat
-from test_adamw_refusals import CS_ERR_ARG, CS_OK, CTensor, _group, _tensor
+from test_adamw_refusals import CS_ERR_ARG, CS_OK, CGrad, CTensor, _group, _tensor
 
 BAD = (dict(exp_avg=None), dict(exp_avg_sq=None), dict(param=None), dict(grad=None))
 
@@ -63,3 +63,23 @@ def test_counted_steps_refuse_missing_counters_and_workspaces(name):
         assert call(good, place=-1) == CS_ERR_ARG
     t[599].exp_avg = None
     assert call(good) == CS_ERR_ARG
+
+
+def test_misaligned_device_scalars_are_refused():
+    g = (type(_group()) * 1)(_group())
+    t = (CTensor * 1)(_tensor())
+    at, gt = ctypes.addressof(t), ctypes.addressof(g)
+    for name, more in (("cs_adamw_step", ()), ("cs_adamw8_step", (7,))):
+        assert nat.call(name, at, 1, gt, 1, None, *more, 66, None) == CS_ERR_ARG  # grad_scale
+        assert nat.call(name, at, 1, gt, 1, 66, *more, None, None) == CS_ERR_ARG  # coef
+        bad = (type(_group()) * 1)(_group(lr_device=66))
+        assert nat.call(name, at, 1, ctypes.addressof(bad), 1, None, *more, None,
+                        None) == CS_ERR_ARG
+    for step, coef in ((260, 64), (256, 66)):
+        steps = (ctypes.c_void_p * 1)(step)
+        assert nat.call("cs_adamw_advance", ctypes.addressof(steps), gt, 1, 0, coef,
+                        None) == CS_ERR_ARG
+    n = (CGrad * 1)(CGrad(256, 1000, 0, 0))
+    for norm, scale in ((66, 64), (64, 66)):
+        assert nat.call("cs_grad_norm", ctypes.addressof(n), 1, 1.0, 1e-6, norm, scale, None,
+                        None) == CS_ERR_ARG
