@@ -65,6 +65,7 @@ struct TensorList {
   TensorList(const TensorList&) = delete;
   TensorList& operator=(const TensorList&) = delete;
   ~TensorList() { Py_XDECREF(fast); }
+  py::object kept() const { return py::reinterpret_borrow<py::object>(fast); }
   std::string at(Py_ssize_t i) const { return std::string(name) + "[" + std::to_string(i) + "]"; }
   const Tensor& operator[](Py_ssize_t i) const {
     if (!THPVariable_Check(items[i])) bad(at(i) + " must be a tensor");
@@ -343,9 +344,10 @@ void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
   }
 }
 
-// A step that has been read and checked and is not yet enqueued.  The caller keeps
-// its tensors.
+// A step that has been read and checked and is not yet enqueued.  It keeps the
+// lists it was read from: an iterator's tensors have no other owner.
 struct Step {
+  std::vector<py::object> lists;
   at::Device dev = at::kCPU;
   int bits;
   Groups r;
@@ -426,6 +428,8 @@ Step read_step(const py::handle& params_, const py::handle& grads_, const py::ha
   }
   set_groups(step.r, step.t);
   step.counters = std::move(counters.at);
+  for (const TensorList* l : {&params, &grads, &m, &v}) step.lists.push_back(l->kept());
+  if (counters.list) step.lists.push_back(counters.list->kept());
   return step;
 }
 
@@ -477,6 +481,8 @@ Step read_step8(const py::handle& params_, const py::handle& grads_, const py::h
   }
   set_groups(step.r, step.t);
   step.counters = std::move(counters.at);
+  for (const TensorList* l : {&params, &grads, &m, &v, &ms, &vs}) step.lists.push_back(l->kept());
+  if (counters.list) step.lists.push_back(counters.list->kept());
   return step;
 }
 

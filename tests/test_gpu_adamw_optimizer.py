@@ -357,3 +357,25 @@ def test_a_learning_rate_saved_from_the_device_and_read_on_the_host():
     assert other.param_groups[0]["lr"].is_cuda
     for p, q in zip(ps, qs):
         assert torch.equal(p, q) and int(other.state[q]["step"]) == 2
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_gradients_from_an_iterator_live_until_the_step_has_run(bits):
+    """Tensors that only the call holds, beside a workspace that it allocates (for a
+    device counter) after it has read them."""
+    runs = []
+    for lazy in (False, True):
+        ps, gen = params_of((4,) * 50 + (3000,), seed=14)
+        ps = [p.detach() for p in ps]
+        base = [make(p.numel(), F32, gen) for p in ps]
+        if bits == 8:
+            state = list(zip(*[ops.adamw8_state(p) for p in ps]))
+        else:
+            state = [[torch.zeros_like(p) for p in ps] for _ in range(2)]
+        count = torch.zeros((), dtype=torch.int64, device="cuda")
+        for _ in range(3):
+            grads = (g * 0.5 for g in base) if lazy else [g * 0.5 for g in base]
+            step = ops.adamw8_step if bits == 8 else ops.adamw_step
+            step(ps, grads, *state, step=count, **HYPER)
+        runs.append(ps)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
