@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <array>
 #include <cmath>
 #include <cstdint>
 #include <optional>
@@ -329,6 +330,7 @@ bool read_param(TensorList& params, TensorList& grads, Py_ssize_t i, const at::D
   if (same_layout(g, p, contiguous) && !g->is_neg()) {
     s.grad = grads.data(g);
   } else {
+    at::NoGradGuard no_grad;
     copies.push_back(at::empty_like(params[i]).copy_(grads[i]));
     s.grad = copies.back().data_ptr();
   }
@@ -347,7 +349,7 @@ void set_groups(const Groups& r, std::vector<cs_adamw_tensor>& t) {
 // A step that has been read and checked and is not yet enqueued.  It keeps the
 // lists it was read from: an iterator's tensors have no other owner.
 struct Step {
-  std::vector<py::object> lists;
+  std::array<py::object, 7> lists;
   at::Device dev = at::kCPU;
   int bits;
   Groups r;
@@ -402,8 +404,6 @@ Step read_step(const py::handle& params_, const py::handle& grads_, const py::ha
   if (params.n == 0) return step;
   step.r = read_groups(groups, params.n, params[0].device());
   const at::Device dev = step.dev = device_of(params);
-  c10::cuda::CUDAGuard guard(dev);
-  at::NoGradGuard no_grad;
   step.scale = device_scalar(grad_scale, dev, "grad_scale");
   step.t.resize(params.n, cs_adamw_tensor{});
   step.changed = step.r.changed;
@@ -428,8 +428,9 @@ Step read_step(const py::handle& params_, const py::handle& grads_, const py::ha
   }
   set_groups(step.r, step.t);
   step.counters = std::move(counters.at);
-  for (const TensorList* l : {&params, &grads, &m, &v}) step.lists.push_back(l->kept());
-  if (counters.list) step.lists.push_back(counters.list->kept());
+  py::object* kept = step.lists.data();
+  for (const TensorList* l : {&params, &grads, &m, &v}) *kept++ = l->kept();
+  if (counters.list) *kept = counters.list->kept();
   return step;
 }
 
@@ -450,8 +451,6 @@ Step read_step8(const py::handle& params_, const py::handle& grads_, const py::h
   if (params.n == 0) return step;
   step.r = read_groups(groups, params.n, params[0].device());
   const at::Device dev = step.dev = device_of(params);
-  c10::cuda::CUDAGuard guard(dev);
-  at::NoGradGuard no_grad;
   step.scale = device_scalar(grad_scale, dev, "grad_scale");
   step.t.resize(params.n, cs_adamw_tensor{});
   step.changed = step.r.changed;
@@ -481,8 +480,9 @@ Step read_step8(const py::handle& params_, const py::handle& grads_, const py::h
   }
   set_groups(step.r, step.t);
   step.counters = std::move(counters.at);
-  for (const TensorList* l : {&params, &grads, &m, &v, &ms, &vs}) step.lists.push_back(l->kept());
-  if (counters.list) step.lists.push_back(counters.list->kept());
+  py::object* kept = step.lists.data();
+  for (const TensorList* l : {&params, &grads, &m, &v, &ms, &vs}) *kept++ = l->kept();
+  if (counters.list) *kept = counters.list->kept();
   return step;
 }
 
