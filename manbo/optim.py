@@ -181,6 +181,13 @@ class AdamW(Optimizer):
             state = {**state, "state": self._loaded}
         super().__setstate__(state)
         self.__dict__.setdefault("grad_norm", None)
+        own = set()  # an optimiser stored by an earlier version shares counters
+        for st in self.state.values():
+            step = st.get("step")
+            if isinstance(step, torch.Tensor):
+                if id(step) in own:
+                    st["step"] = step.clone()
+                own.add(id(st["step"]))
         for group in self.param_groups:
             for key, value in self.defaults.items():
                 group.setdefault(key, value)

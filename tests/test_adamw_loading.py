@@ -178,3 +178,15 @@ def test_learning_rates_that_are_tensors():
                         .state_dict())
     assert [g["lr"] for g in new.param_groups] == [0.125, 0.125, 0.5]
     assert type(new.param_groups[0]["lr"]) is float
+
+
+def test_stored_optimisers_whose_parameters_share_a_counter_get_one_each():
+    ps = [torch.zeros(3, requires_grad=True) for _ in range(3)]
+    opt = manbo.AdamW(ps, capturable=True)
+    shared = torch.tensor(5)
+    for p in ps[:2]:
+        opt.state[p] = dict(exp_avg=torch.zeros(3), exp_avg_sq=torch.zeros(3), step=shared)
+    other = copy.deepcopy(opt)
+    a, b = (other.state[p]["step"] for p in other.param_groups[0]["params"][:2])
+    a += 1
+    assert int(a) == 6 and int(b) == 5 and int(shared) == 5
