@@ -379,3 +379,85 @@ def test_gradients_from_an_iterator_live_until_the_step_has_run(bits):
             step(ps, grads, *state, step=count, **HYPER)
         runs.append(ps)
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_non_finite_gradients_of_unaligned_parameters(dtype, shift):
+    """Every path of a block (aligned, by way of shared memory, cut short): the
+    element's parameter and the whole block's moments."""
+    n = 256 * 5 + 100
+    p = torch.ones(n + shift, dtype=dtype, device="cuda")[shift:]
+    g = torch.full((n + shift,), 0.1, dtype=dtype, device="cuda")[shift:]
+    st = ops.adamw8_state(p)
+    bad = {3: float("nan"), 700: float("inf"), n - 1: -float("inf")}
+    for i, x in bad.items():
+        g[i] = x
+    ops.adamw8_step([p], [g], *[[x] for x in st], step=1, **HYPER)
+    assert [e == 255 for e in st[1].tolist()] == [b in (0, 2, 5) for b in range(6)]
+    assert [e == 255 for e in st[3].tolist()] == [b in (0, 2, 5) for b in range(6)]
+    assert torch.isnan(p).nonzero().view(-1).tolist() == sorted(bad)
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    p = torch.ones(n + shift, dtype=dtype, device="cuda")[shift:]
+    ops.adamw_step([p], [g], [m], [v], step=1, **HYPER)
+    assert torch.isnan(p).nonzero().view(-1).tolist() == sorted(bad)
+    assert (~torch.isfinite(m)).nonzero().view(-1).tolist() == sorted(bad)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 0.0])
+def test_grad_scales_that_are_not_ordinary(scale):
+    """NaN and infinity reach every parameter (0 times infinity is NaN, and the first
+    step of an infinite average is infinity over infinity), zero none."""
+    c = torch.tensor(scale, device="cuda")
+    p, g = torch.ones(600, device="cuda"), torch.full((600,), 0.1, device="cuda")
+    g[5] = 0
+    m, v = torch.zeros(600, device="cuda"), torch.zeros(600, device="cuda")
+    ops.adamw_step([p], [g], [m], [v], step=1, grad_scale=c, **HYPER)
+    q = torch.ones(600, device="cuda")
+    st = ops.adamw8_state(q)
+    ops.adamw8_step([q], [g], *[[x] for x in st], step=1, grad_scale=c, **HYPER)
+    if scale == 0.0:
+        assert not m.any() and not v.any() and not st[0].any() and not st[2].any()
+        assert torch.equal(p, q) and torch.isfinite(p).all()
+    else:
+        assert torch.isnan(p).all() and torch.isnan(q).all()
+        assert (st[1] == 255).all() and (st[3] == 255).all()
+
+
+def test_a_closure_runs_with_gradients_and_gives_the_loss():
+    p = torch.ones(5, device="cuda", requires_grad=True)
+    opt = manbo.AdamW([p], lr=0.1, weight_decay=0.0)
+
+    def closure():
+        opt.zero_grad()
+        loss = (p * p).sum()
+        loss.backward()
+        return loss
+    assert float(opt.step(closure).detach()) == 5.0
+    # the first step moves by lr against the gradient's sign; eps and roundings: 1e-6
+    assert float((p - 0.9).abs().max()) < 1e-6
+
+
+def test_float32_tensors_of_many_chunks_a_cta():
+    """60 M float32 elements: four and more blocks a warp, without the prefetch
+    that 16-bit parameters have; windows against the restatement."""
+    n = 60_000_077
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    p = torch.randn(n, device="cuda", generator=gen) * 0.3
+    g = torch.randn(n, device="cuda", generator=gen) * 1e-2
+    st = ops.adamw8_state(p)
+    ops.adamw8_step([p], [g], *[[x] for x in st], step=1, seed=3, **HYPER)
+    blocks, chunks = -(-n // 256), -(-n // 1024)
+    starts = {0, blocks - 3, blocks // 2}
+    for per in (2, 4, 8, 16, 32):
+        stride = -(-chunks // per) * 4
+        starts |= {b for b in (stride - 2, stride * (per - 1) - 1) if 0 <= b < blocks - 3}
+    for b in sorted(starts):
+        at, end = b * 256, min(n, (b + 3) * 256)
+        zeros, scales = np.zeros(end - at, np.uint8), np.zeros(-(-(end - at) // 256), np.uint8)
+        new = oa.step8(g[at:end].cpu().numpy(), zeros, scales, zeros, scales, step=1,
+                       betas=HYPER["betas"], seed=3, first_block=b)
+        for got, want in zip((st[0][at:end], st[1][b:b + 3], st[2][at:end], st[3][b:b + 3]),
+                             new[2:]):
+            np.testing.assert_array_equal(got.cpu().numpy(), want)
+    assert int((st[0] == 0).sum()) < n // 1000 and not (st[1] == 0).any()
