@@ -5,8 +5,8 @@ for the render/optimise hot path: the cubic fill and stroke renderers, their
 per-stage operators, the ring-segment conversion, the MSE / PSNR / SSIM
 metrics, the Adan optimiser that train.py uses by default, the regularisation
 loss and the connected-component labelling; and, beside the reference's names,
-an AdamW optimiser that moves all parameters in one launch.  The Gaussian renderer, outside
-that path, keeps its names so that imports succeed, and raises
+an AdamW optimiser that moves many parameters in one launch.  The Gaussian
+renderer, outside that path, keeps its names so that imports succeed, and raises
 NotImplementedError when called.
 """
 import importlib.util as _ilu

@@ -1,8 +1,8 @@
 """AdamW over many tensors at once, on the B200 kernels.
 
 ``grad_norm`` is the global 2-norm of a list of gradients with its clip factor,
-both left on the device; ``adamw_step`` moves a whole list of parameters in one
-launch, ``adamw8_step`` does so with moments of one byte an element, and
+both left on the device; ``adamw_step`` moves a list of parameters, several
+hundred a launch, ``adamw8_step`` does so with moments of one byte an element, and
 ``adamw8_moments`` gives the values those bytes stand for.  The reference has
 none of them: its optimisers are Adan (``adan_step_from_grad_tilelang``) and
 torch's Adam, one parameter at a time, with the clip factor read on the host.
@@ -37,12 +37,13 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *, step,
                lr=1e-3, betas: tuple = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, grad_scale: torch.Tensor | None = None) -> None:
-    """One AdamW step in place, every tensor in one launch.
+    """One AdamW step in place, several hundred tensors a launch.
 
     With g' = grad_scale g: m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2,
     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
     The moments are float32 in the parameter's layout.  ``step`` is t (an int
-    from 1) or an int64 device counter, which the call advances and then uses;
+    from 1) or an int64 device counter, which the call advances and then uses (an
+    empty list moves nothing and counts nothing);
     ``lr`` a float or a float32 device scalar; ``grad_scale`` a float32 device
     scalar such as ``grad_norm`` returns.  A 16-bit parameter is rounded to the
     nearest value once, at the end.

@@ -7,9 +7,9 @@ gradient-norm clipping as the reference; every parameter's update is one
 ``cs_adan_step`` launch.  Like the reference, clipping (max_grad_norm > 0)
 reads the norm on the host, once per step.
 
-``AdamW`` (no counterpart in the reference) moves every parameter in one launch,
-with its moments in 32 bits or in 8 (manbo/ops/adamw.py), clips by the global
-gradient norm without reading it back, and can be captured in a CUDA graph.
+``AdamW`` (no counterpart in the reference) moves several hundred parameters a
+launch, with its moments in 32 bits or in 8 (manbo/ops/adamw.py), clips by the
+global gradient norm without reading it back, and can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
@@ -136,7 +136,10 @@ def _order(t):
 
 
 class AdamW(Optimizer):
-    """Adam with decoupled weight decay, every parameter of a device in one launch.
+    """Adam with decoupled weight decay, several hundred parameters a launch.
+
+    A launch holds one device, ``state_bits``, ``seed`` and ``capturable``, and up to
+    16 pairs of group and step number.
 
     ``state_bits`` 32 keeps ``exp_avg`` and ``exp_avg_sq`` as float32 in the
     parameter's layout, 8 as one byte an element with a scale byte for each 256
