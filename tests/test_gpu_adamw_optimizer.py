@@ -435,7 +435,7 @@ def test_a_closure_runs_with_gradients_and_gives_the_loss():
         return loss
     assert float(opt.step(closure).detach()) == 5.0
     # the first step moves by lr against the gradient's sign; eps and roundings: 1e-6
-    assert float((p - 0.9).abs().max()) < 1e-6
+    assert float((p.detach() - 0.9).abs().max()) < 1e-6
 
 
 def test_float32_tensors_of_many_chunks_a_cta():
@@ -461,3 +461,35 @@ def test_float32_tensors_of_many_chunks_a_cta():
                              new[2:]):
             np.testing.assert_array_equal(got.cpu().numpy(), want)
     assert int((st[0] == 0).sum()) < n // 1000 and not (st[1] == 0).any()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_empty_parameters_are_counted_and_nothing_else(bits, capturable):
+    ps = [torch.zeros(n, device="cuda", requires_grad=True) for n in (0, 5, 0)]
+    opt = manbo.AdamW(ps, state_bits=bits, capturable=capturable, max_grad_norm=1.0)
+    for t in (1, 2, 3):
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        if t == 3:
+            ps[1].grad = None  # nothing to move at all
+        opt.step()
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 2, 3]
+    assert float(opt.grad_norm) == 0.0 and bool((ps[1] < 0).all())
+
+
+def test_counted_8_bit_steps_of_many_parameters_round_as_the_restatement():
+    """More tensors than a table and than a launch of counters take."""
+    ps, gen = params_of([1 + (i * 7) % 600 for i in range(900)], seed=15)
+    opt = manbo.AdamW(ps, state_bits=8, capturable=True, seed=21)
+    state = [(np.zeros(p.numel(), np.uint8), np.zeros(-(-p.numel() // 256), np.uint8)) * 2
+             for p in ps]
+    for t in (1, 2):
+        for i, p in enumerate(ps):
+            p.grad = make(p.numel(), F32, gen)
+            state[i] = oa.step8(p.grad.cpu().numpy(), *state[i], step=t, seed=21, place=i)[2:]
+        opt.step()
+    for p, want in zip(ps, state):
+        st = opt.state[p]
+        for k, w in zip(("exp_avg", "exp_avg_scales", "exp_avg_sq", "exp_avg_sq_scales"), want):
+            np.testing.assert_array_equal(st[k].cpu().numpy(), w)
