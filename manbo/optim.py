@@ -194,6 +194,9 @@ class AdamW(Optimizer):
         for group in self.param_groups:
             for key, value in self.defaults.items():
                 group.setdefault(key, value)
+        # one value for all groups, those that are added later among them
+        if len({group["max_grad_norm"] for group in self.param_groups}) == 1:
+            self.defaults["max_grad_norm"] = self.param_groups[0]["max_grad_norm"]
 
     def _new_state(self, p, group, capturing):
         if capturing:

@@ -190,3 +190,12 @@ def test_stored_optimisers_whose_parameters_share_a_counter_get_one_each():
     a, b = (other.state[p]["step"] for p in other.param_groups[0]["params"][:2])
     a += 1
     assert int(a) == 6 and int(b) == 5 and int(shared) == 5
+
+
+def test_a_group_added_after_a_load_clips_with_the_others():
+    ps = [torch.zeros(3, requires_grad=True) for _ in range(2)]
+    old = manbo.AdamW(ps[:1], max_grad_norm=0.5)
+    new = manbo.AdamW(ps[:1])
+    new.load_state_dict(old.state_dict())
+    new.add_param_group({"params": ps[1:]})
+    assert [g["max_grad_norm"] for g in new.param_groups] == [0.5, 0.5]
